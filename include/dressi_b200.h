@@ -322,6 +322,102 @@ int dressi_avg_pool2x2_grad(const float* gy, uint32_t w, uint32_t h,
                             uint32_t n_comp, float* g_x, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Learning operators (extensions: the reference has no counterpart): a
+ * normalisation layer over channels-last images and an optimiser step over
+ * many tensors
+ * --------------------------------------------------------------------- */
+
+/* element types of the tensors below */
+#define DRESSI_F32 0
+#define DRESSI_F16 1
+#define DRESSI_BF16 2
+
+/* activations of dressi_group_norm */
+#define DRESSI_ACT_NONE 0
+#define DRESSI_ACT_RELU 1
+#define DRESSI_ACT_SILU 2
+
+typedef struct dressi_group_norm_desc {
+    uint32_t struct_size; /* sizeof(dressi_group_norm_desc) */
+    int32_t dtype;        /* of x, y, dy and dx */
+    int32_t activation;
+    uint32_t channels, groups; /* groups divides channels */
+    float eps;
+    uint64_t n, rows; /* x [n][rows][channels]: rows = height * width */
+} dressi_group_norm_desc;
+
+/* Bytes of device workspace of a forward (grad = 0) or backward (1) call. */
+int dressi_group_norm_workspace(const dressi_group_norm_desc* d, int grad,
+                                size_t* bytes);
+
+/* y = act((x - mean) * rstd * weight + bias), the mean and the (biased)
+ * variance over a sample's rows and a group's channels. weight / bias
+ * [channels] f32 or NULL (1 / 0). mean / rstd [n][groups] f32 receive the
+ * statistics (both or neither NULL). Images are aligned to their element,
+ * the workspace to 16 bytes; its contents do not matter. y must not overlap
+ * x. */
+int dressi_group_norm(const dressi_group_norm_desc* d, const void* x,
+                      const float* weight, const float* bias, void* y,
+                      float* mean, float* rstd, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The gradients for dy, from x and the statistics of the forward call. dx,
+ * dweight and dbias are overwritten; each may be NULL. Repeats bit for bit. */
+int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
+                           const void* x, const float* weight,
+                           const float* bias, const float* mean,
+                           const float* rstd, void* dx, float* dweight,
+                           float* dbias, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* The fewest bytes of workspace of dressi_grad_norm. */
+int dressi_grad_norm_workspace(size_t* bytes);
+
+/* out[0] = sqrt(sum of squares over n_tensors tensors), summed in 64 bits in
+ * an order that the sizes alone give. tensors, numel and dtypes are host
+ * arrays (read before the call returns) of device addresses, lengths and
+ * element types. The workspace is aligned to 8 bytes. */
+int dressi_grad_norm(uint32_t n_tensors, const void* const* tensors,
+                     const uint64_t* numel, const int32_t* dtypes, float* out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step of n_tensors tensors (distinct, each with its own state):
+ *   g *= min(1, max_norm / (*grad_norm + 1e-6))     if max_norm > 0
+ *   m = m b1 + g (1 - b1);  v = v b2 + g g (1 - b2);  t = t + 1
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ *   p = min(max(p, clamp_lo), clamp_hi)
+ * The arrays are host arrays, read before the call returns. With
+ * state_bits = 8, blocks of 256 values of a tensor hold e4m3 codes of m and
+ * of sqrt(v) and a scale each (value = code * scale), rounded up or down at
+ * random with the right mean; the random bits come from (seed, t, index,
+ * place), so a step repeats exactly. All state starts as zeros. */
+typedef struct dressi_adamw_desc {
+    uint32_t struct_size; /* sizeof(dressi_adamw_desc) */
+    uint32_t n_tensors;
+    int32_t dtype;      /* of parameters and gradients */
+    int32_t state_bits; /* 32 or 8 */
+    const uint64_t* numel;
+    void* const* params;
+    const void* const* grads;
+    void* const* exp_avg;         /* f32 [numel], or codes [numel] */
+    void* const* exp_avg_sq;      /* f32 [numel], or codes of the root */
+    float* const* exp_avg_scale;  /* 8 bits: [ceil(numel / 256)] */
+    float* const* exp_avg_sq_scale;
+    int32_t* const* steps; /* a device counter for each tensor */
+    const uint32_t* index; /* a number for each tensor, or NULL (its place) */
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* lr_device; /* device scalar in place of lr, or NULL */
+    double max_norm;        /* 0: no clipping */
+    const float* grad_norm; /* device scalar; with max_norm */
+    float clamp_lo, clamp_hi; /* -inf / inf: no clamp */
+    uint32_t seed;
+    uint32_t* ticket; /* device word, zeroed once by the caller; 0 again after
+                         every call. Calls that overlap need one each. */
+} dressi_adamw_desc;
+
+int dressi_adamw_step(const dressi_adamw_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------
  * Indexed access of the paper's HardSoftRas (f_ops.cpp:1490-1799). Device
  * pointers, float ids (the reference's leaves), n_comp 1..4; each output is
  * written. A table id out of range sets DRESSI_STATUS_INDEX_RANGE in

@@ -58,6 +58,41 @@ class AaSilhouetteDesc(C.Structure):
     ]
 
 
+# element types and activations of the learning operators
+F32, F16, BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+
+
+class GroupNormDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32), ("activation", C.c_int32),
+        ("channels", C.c_uint32), ("groups", C.c_uint32),
+        ("eps", C.c_float),
+        ("n", C.c_uint64), ("rows", C.c_uint64),
+    ]
+
+
+class AdamWDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("n_tensors", C.c_uint32),
+        ("dtype", C.c_int32), ("state_bits", C.c_int32),
+        # host arrays
+        ("numel", C.c_void_p), ("params", C.c_void_p), ("grads", C.c_void_p),
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+        ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p),
+        ("steps", C.c_void_p), ("index", C.c_void_p),
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+        ("eps", C.c_double), ("weight_decay", C.c_double),
+        ("lr_device", C.c_void_p),
+        ("max_norm", C.c_double), ("grad_norm", C.c_void_p),
+        ("clamp_lo", C.c_float), ("clamp_hi", C.c_float),
+        ("seed", C.c_uint32),
+        ("ticket", C.c_void_p),
+    ]
+
+
 class PbrDesc(C.Structure):
     _fields_ = [
         ("struct_size", C.c_uint32),
@@ -199,6 +234,19 @@ SIGNATURES = {
                                       C.POINTER(C.c_char_p), _fp,
                                       C.POINTER(_u32), C.POINTER(_u32)]),
     "dressi_plan_destroy": (C.c_int, [_vp]),
+    # learning operators
+    "dressi_group_norm_workspace": (C.c_int, [C.POINTER(GroupNormDesc),
+                                              C.c_int,
+                                              C.POINTER(C.c_size_t)]),
+    "dressi_group_norm": (C.c_int, [C.POINTER(GroupNormDesc), _vp, _vp, _vp,
+                                    _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "dressi_group_norm_grad": (C.c_int, [C.POINTER(GroupNormDesc), _vp, _vp,
+                                         _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                         _vp, C.c_size_t, _vp]),
+    "dressi_grad_norm_workspace": (C.c_int, [C.POINTER(C.c_size_t)]),
+    "dressi_grad_norm": (C.c_int, [_u32, _vp, _vp, _vp, _vp, _vp, C.c_size_t,
+                                   _vp]),
+    "dressi_adamw_step": (C.c_int, [C.POINTER(AdamWDesc), _vp]),
     # graph path
     "dressi_var_create": (C.c_int, [C.c_int, _u32, _u32, C.POINTER(_vp)]),
     "dressi_var_clone": (C.c_int, [_vp, C.POINTER(_vp)]),

@@ -1,0 +1,605 @@
+// AdamW over many tensors in one launch, its moments in 32 or in 8 bits, and
+// the norm over many tensors that it clips by (an extension: the reference
+// steps one image per in-graph Adam).
+//
+//   m = m b1 + g (1 - b1);  v = v b2 + g g (1 - b2);  t = t + 1
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// with g first scaled by min(1, max_norm / (norm + 1e-6)) when clipping, and p
+// clamped last. Every operation is rounded by itself, as in the plans' Adam.
+// Bound by memory: 28 bytes a value with f32 parameters and 32-bit moments,
+// 16 + 8/256 with 8-bit ones.
+//
+// The tensors' addresses travel as a kernel argument (no table to upload, so
+// a step can be captured), the work is cut into blocks of 256 values of one
+// tensor, a warp each, and every thread block takes an equal contiguous run of
+// them. Step counters live on the device, one per tensor: the last thread
+// block of a launch to finish adds one to each.
+//
+// 8-bit moments. Each block of 256 holds e4m3 codes of m and of r = sqrt(v)
+// (v itself would need twice the exponent range) and a scale each, the
+// largest |value| / 448. A moving average moves by far less than the half step
+// of an 8-bit format in one step (0.05% against 6%), so rounding to the
+// nearest would hold it where it is: values are rounded up or down with the
+// probability of their place between the two neighbours. The 16 random bits
+// for each come from Wang's hash of (seed, step, tensor, place), so a run
+// repeats exactly. r > 0 is never rounded to 0: m / (0 + eps) would explode.
+// What is not finite is stored as NaN and leaves the block's scale alone.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "exact.cuh"
+#include "kernels.h"
+
+namespace dressi {
+
+namespace {
+
+constexpr int kBlock = 256;    // values a warp takes, and that share a scale
+constexpr int kLane = 8;       // values a lane takes
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kCtasPerSm = 4;
+constexpr uint32_t kNone = 0xffffffffu;
+constexpr uint64_t kMostBlocks = 1ull << 31;  // of one launch
+
+struct AdamWHyper {
+    float b1, omb1, b2, omb2, eps, ln_b1, ln_b2;
+    float lo, hi, max_norm;
+    double lr, wd;
+    const float* lr_device;
+    const float* norm;
+    uint32_t seed;
+    uint32_t* ticket;
+};
+
+// The tensors of a launch; 400 fill the 32764 bytes of a kernel's arguments.
+template <int CAP>
+struct AdamWTable {
+    void* p[CAP];
+    const void* g[CAP];
+    void* m[CAP];
+    void* v[CAP];
+    float* sm[CAP];
+    float* sv[CAP];
+    int32_t* step[CAP];
+    uint64_t n[CAP];
+    uint32_t first[CAP + 1];  // block that the tensor begins with
+    uint32_t index[CAP];
+    uint8_t wide[CAP];  // aligned for whole-lane loads and stores
+    uint32_t count;
+};
+
+struct alignas(32) F8 {
+    float v[8];
+};
+
+__device__ __forceinline__ void load8(const float* p, float* o) {
+    const F8 a = *reinterpret_cast<const F8*>(p);
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = a.v[j];
+}
+__device__ __forceinline__ void store8(float* p, const float* o) {
+    F8 a;
+#pragma unroll
+    for (int j = 0; j < 8; j++) a.v[j] = o[j];
+    *reinterpret_cast<F8*>(p) = a;
+}
+__device__ __forceinline__ void load8(const __half* p, float* o) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const __half2* h = reinterpret_cast<const __half2*>(&a);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        o[2 * j] = __low2float(h[j]);
+        o[2 * j + 1] = __high2float(h[j]);
+    }
+}
+__device__ __forceinline__ void store8(__half* p, const float* o) {
+    uint4 a;
+    __half2* h = reinterpret_cast<__half2*>(&a);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        h[j] = __floats2half2_rn(o[2 * j], o[2 * j + 1]);
+    *reinterpret_cast<uint4*>(p) = a;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* o) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t* h = reinterpret_cast<const uint32_t*>(&a);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        o[2 * j] = __uint_as_float(h[j] << 16);
+        o[2 * j + 1] = __uint_as_float(h[j] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* o) {
+    uint4 a;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&a);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        h[j] = __floats2bfloat162_rn(o[2 * j], o[2 * j + 1]);
+    *reinterpret_cast<uint4*>(p) = a;
+}
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) {
+    return __bfloat162float(v);
+}
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) {
+    *p = __float2half_rn(v);
+}
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) {
+    *p = __float2bfloat16_rn(v);
+}
+
+// The 8 values of a lane: consecutive ones where the block is whole and
+// aligned, else those at lane + 32 j with j's bit of `mask` set.
+template <typename T>
+__device__ __forceinline__ void load_lane(const T* p, bool wide, uint32_t mask,
+                                          int lane, float* o) {
+    if (wide) {
+        load8(p + lane * kLane, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane; j++)
+            o[j] = mask >> j & 1 ? to_f(p[lane + 32 * j]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_lane(T* p, bool wide, uint32_t mask,
+                                           int lane, const float* o) {
+    if (wide) {
+        store8(p + lane * kLane, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane; j++)
+            if (mask >> j & 1) put(p + lane + 32 * j, o[j]);
+    }
+}
+
+// e4m3 codes of a lane (packed) and the values they stand for.
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, bool wide,
+                                            uint32_t mask, int lane) {
+    if (wide) return *reinterpret_cast<const uint2*>(p + lane * kLane);
+    uint32_t c[2] = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < kLane; j++)
+        if (mask >> j & 1)
+            c[j / 4] |= uint32_t(p[lane + 32 * j]) << (j % 4 * 8);
+    return make_uint2(c[0], c[1]);
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, bool wide,
+                                            uint32_t mask, int lane, uint2 c) {
+    if (wide) {
+        *reinterpret_cast<uint2*>(p + lane * kLane) = c;
+        return;
+    }
+    const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+    for (int j = 0; j < kLane; j++)
+        if (mask >> j & 1)
+            p[lane + 32 * j] = uint8_t(w[j / 4] >> (j % 4 * 8));
+}
+__device__ __forceinline__ void decode(uint2 c, float* o) {
+    const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const __half2 h(__nv_cvt_fp8x2_to_halfraw2(
+                __nv_fp8x2_storage_t(w[j / 2] >> (j % 2 * 16)), __NV_E4M3));
+        o[2 * j] = __low2float(h);
+        o[2 * j + 1] = __high2float(h);
+    }
+}
+
+// The scale of a block's 8-bit values and 1 over it, from the largest finite
+// |x| of the warp. The floor keeps 448 / top finite.
+__device__ __forceinline__ float top_of(const float* x, bool* finite) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int j = 0; j < kLane; j++)
+        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    *finite = top < 0x7f800000u;
+    if (!*finite) {
+        top = 0u;
+#pragma unroll
+        for (int j = 0; j < kLane; j++) {
+            const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
+            top = max(top, b < 0x7f800000u ? b : 0u);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+    }
+    return fmaxf(__uint_as_float(top), 0x1p-100f);
+}
+
+// a >= 0 up or down to a neighbouring e4m3 value, up with the probability of
+// its place between the two: 16 random bits (and a half) are added below the
+// 3 bits of fraction that stay. Below 2^-6 the values are 2^-9 apart, as they
+// are in [2^-6, 2^-5): the sum with 2^-6 is rounded instead.
+__device__ __forceinline__ float round_e4m3(float a, uint32_t bits16) {
+    const float lift = a < 0x1p-6f ? 0x1p-6f : 0.f;
+    const uint32_t b = __float_as_uint(a + lift) + (bits16 << 4 | 8u);
+    return fminf(__uint_as_float(b & 0xfff00000u) - lift, 448.f);
+}
+
+// The codes of a lane's values x; ROOT: of values that are not negative and
+// do not become 0 unless they are.
+template <bool ROOT>
+__device__ __forceinline__ uint2 encode(const float* x, float inv, bool finite,
+                                        const uint32_t* bits) {
+    uint32_t w[2] = {0u, 0u};
+    float a[kLane];
+#pragma unroll
+    for (int j = 0; j < kLane; j++) {
+        a[j] = round_e4m3(fminf(fabsf(x[j]) * inv, 448.f),
+                          ROOT ? bits[j] >> 16 : bits[j] & 0xffffu);
+        if (ROOT) {
+            a[j] = x[j] > 0.f ? fmaxf(a[j], 0x1p-9f) : a[j];
+        } else {
+            a[j] = copysignf(a[j], x[j]);
+        }
+    }
+    if (!finite) {
+#pragma unroll
+        for (int j = 0; j < kLane; j++)
+            if ((__float_as_uint(x[j]) & 0x7f800000u) == 0x7f800000u)
+                a[j] = __uint_as_float(0x7fc00000u);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        w[j / 2] |= uint32_t(__nv_cvt_float2_to_fp8x2(
+                            make_float2(a[2 * j], a[2 * j + 1]),
+                            __NV_SATFINITE, __NV_E4M3))
+                    << (j % 2 * 16);
+    return make_uint2(w[0], w[1]);
+}
+
+// The tensor whose blocks block b is among.
+template <typename Table>
+__device__ __forceinline__ uint32_t tensor_of(const Table& t, uint32_t b) {
+    uint32_t lo = 0, hi = t.count;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (t.first[mid] <= b) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T, int BITS, int CAP>
+__global__ void __launch_bounds__(kThreads)
+        k_adamw(const __grid_constant__ AdamWTable<CAP> t,
+                const __grid_constant__ AdamWHyper h) {
+    const int lane = threadIdx.x & 31;
+    const uint64_t all = t.first[t.count];
+    const uint32_t b_end = uint32_t(all * (blockIdx.x + 1) / gridDim.x);
+    uint32_t b = uint32_t(all * blockIdx.x / gridDim.x) + threadIdx.x / 32;
+
+    float scale = 1.f;  // of the gradients
+    if (h.norm) {
+        const float c = h.max_norm / (*h.norm + 1e-6f);
+        scale = c > 1.f ? 1.f : c;  // NaN stays
+    }
+    const double lr = h.lr_device ? double(*h.lr_device) : h.lr;
+    const float decay = float(1.0 - lr * h.wd);
+
+    uint32_t ti = kNone, key = 0;
+    float size = 0.f, root = 0.f;
+    for (; b < b_end; b += kWarps) {
+        if (ti == kNone || b >= t.first[ti + 1]) {
+            if (ti == kNone) ti = tensor_of(t, b);
+            while (b >= t.first[ti + 1]) ti++;
+            const int32_t step = *t.step[ti] + 1;
+            // 1 - b^t = -expm1(t ln b): exact to a few 2^-24, also where b^t
+            // is next to 1
+            size = float(lr / double(-expm1f(float(step) * h.ln_b1)));
+            root = 1.f / sqrtf(-expm1f(float(step) * h.ln_b2));
+            if (BITS == 8)
+                key = wang_hash(wang_hash(h.seed ^ wang_hash(uint32_t(step))) +
+                                t.index[ti]);
+        }
+        const uint64_t at = uint64_t(b - t.first[ti]) * kBlock;
+        const uint64_t left = t.n[ti] - at;
+        const bool wide = t.wide[ti] && left >= kBlock;
+        uint32_t mask = 0xffu;
+        if (!wide && left < kBlock) {
+            mask = 0u;
+#pragma unroll
+            for (int j = 0; j < kLane; j++)
+                mask |= uint32_t(lane + 32 * j < int(left)) << j;
+        }
+        T* pp = static_cast<T*>(t.p[ti]) + at;
+        float p[kLane], g[kLane], m[kLane], v[kLane];
+        load_lane(static_cast<const T*>(t.g[ti]) + at, wide, mask, lane, g);
+        load_lane(static_cast<const T*>(pp), wide, mask, lane, p);
+        if (BITS == 32) {
+            load_lane(static_cast<const float*>(t.m[ti]) + at, wide, mask,
+                      lane, m);
+            load_lane(static_cast<const float*>(t.v[ti]) + at, wide, mask,
+                      lane, v);
+        } else {
+            const uint32_t q = b - t.first[ti];
+            const uint2 cm = load_codes(
+                    static_cast<const uint8_t*>(t.m[ti]) + at, wide, mask,
+                    lane);
+            const uint2 cv = load_codes(
+                    static_cast<const uint8_t*>(t.v[ti]) + at, wide, mask,
+                    lane);
+            const float sm = t.sm[ti][q], sv = t.sv[ti][q];
+            decode(cm, m);
+            decode(cv, v);
+#pragma unroll
+            for (int j = 0; j < kLane; j++) {
+                m[j] = m[j] * sm;
+                v[j] = v[j] * sv;
+                v[j] = v[j] * v[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kLane; j++) {
+            const float gj = g[j] * scale;
+            m[j] = m[j] * h.b1 + gj * h.omb1;
+            v[j] = v[j] * h.b2 + (gj * gj) * h.omb2;
+            const float r = sqrtf(v[j]);
+            float q = p[j] * decay - size * (m[j] / (r * root + h.eps));
+            q = q < h.lo ? h.lo : q;  // NaN stays
+            p[j] = q > h.hi ? h.hi : q;
+            if (BITS == 8) v[j] = r;
+        }
+        store_lane(pp, wide, mask, lane, p);
+        if (BITS == 32) {
+            store_lane(static_cast<float*>(t.m[ti]) + at, wide, mask, lane, m);
+            store_lane(static_cast<float*>(t.v[ti]) + at, wide, mask, lane, v);
+        } else {
+            const uint32_t q = b - t.first[ti];
+            uint32_t bits[kLane];
+#pragma unroll
+            for (int j = 0; j < kLane; j++)
+                bits[j] = wang_hash(key + uint32_t(at) +
+                                    (wide ? lane * kLane + j : lane + 32 * j));
+            bool fm, fv;
+            const float tm = top_of(m, &fm), tv = top_of(v, &fv);
+            store_codes(static_cast<uint8_t*>(t.m[ti]) + at, wide, mask, lane,
+                        encode<false>(m, 448.f / tm, fm, bits));
+            store_codes(static_cast<uint8_t*>(t.v[ti]) + at, wide, mask, lane,
+                        encode<true>(v, 448.f / tv, fv, bits));
+            if (lane == 0) {
+                t.sm[ti][q] = tm / 448.f;
+                t.sv[ti][q] = tv / 448.f;
+            }
+        }
+    }
+    // every block has read the counters once all have drawn a ticket
+    __shared__ bool last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(h.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (last) {
+        for (uint32_t i = threadIdx.x; i < t.count; i += kThreads)
+            *t.step[i] += 1;
+        if (threadIdx.x == 0) *h.ticket = 0u;
+    }
+}
+
+int sm_count() {
+    int dev = 0, sms = 148;
+    DRESSI_CUDA(cudaGetDevice(&dev));
+    DRESSI_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount,
+                                       dev));
+    return sms;
+}
+
+bool aligned(const void* p, size_t a) {
+    return reinterpret_cast<uintptr_t>(p) % a == 0;
+}
+
+template <typename T, int BITS, int CAP>
+void launch_adamw(const AdamWArgs& a, const AdamWHyper& h, uint32_t i0,
+                  uint32_t i1, cudaStream_t s) {
+    AdamWTable<CAP> t;
+    t.count = i1 - i0;
+    uint64_t blocks = 0;
+    for (uint32_t i = i0; i < i1; i++) {
+        const uint32_t k = i - i0;
+        t.p[k] = a.params[i];
+        t.g[k] = a.grads[i];
+        t.m[k] = a.exp_avg[i];
+        t.v[k] = a.avg_sq[i];
+        t.sm[k] = BITS == 8 ? a.exp_avg_scale[i] : nullptr;
+        t.sv[k] = BITS == 8 ? a.avg_sq_scale[i] : nullptr;
+        t.step[k] = a.steps[i];
+        t.n[k] = a.numel[i];
+        t.index[k] = a.index ? a.index[i] : i;
+        const size_t st = BITS == 8 ? kLane : kLane * sizeof(float);
+        t.wide[k] = aligned(t.p[k], kLane * sizeof(T)) &&
+                    aligned(t.g[k], kLane * sizeof(T)) &&
+                    aligned(t.m[k], st) && aligned(t.v[k], st);
+        t.first[k] = uint32_t(blocks);
+        blocks += (t.n[k] + kBlock - 1) / kBlock;
+    }
+    t.first[t.count] = uint32_t(blocks);
+    const uint64_t grid = std::max<uint64_t>(
+            1, std::min<uint64_t>((blocks + kWarps - 1) / kWarps,
+                                  uint64_t(sm_count()) * kCtasPerSm));
+    k_adamw<T, BITS, CAP><<<unsigned(grid), kThreads, 0, s>>>(t, h);
+    DRESSI_CUDA(cudaGetLastError());
+}
+
+template <typename T, int BITS>
+void adamw_t(const AdamWArgs& a, const AdamWHyper& h, cudaStream_t s) {
+    constexpr uint32_t kFew = 32, kMany = 400;
+    for (uint32_t i0 = 0; i0 < a.n_tensors;) {
+        uint32_t i1 = i0;
+        uint64_t blocks = 0;
+        while (i1 < a.n_tensors && i1 - i0 < kMany) {
+            const uint64_t more = (a.numel[i1] + kBlock - 1) / kBlock;
+            if (i1 > i0 && blocks + more > kMostBlocks) break;
+            blocks += more;
+            i1++;
+        }
+        if (i1 - i0 <= kFew) launch_adamw<T, BITS, kFew>(a, h, i0, i1, s);
+        else launch_adamw<T, BITS, kMany>(a, h, i0, i1, s);
+        i0 = i1;
+    }
+}
+
+// --------------------------------------------------------------------- norm
+
+constexpr int kNormCap = 1000;
+constexpr int kNormUnit = kThreads * kLane;  // values a thread block takes
+constexpr int kNormCtasPerSm = 4;
+constexpr int kNormMost = 1024;              // thread blocks (partial sums)
+
+struct NormTable {
+    const void* p[kNormCap];
+    uint64_t n[kNormCap];
+    uint32_t first[kNormCap + 1];
+    uint8_t type[kNormCap];
+    uint32_t count;
+};
+
+// Squares are summed in 64 bits from the first on: no overflow, and an order
+// that depends on the sizes alone.
+template <typename T>
+__device__ __forceinline__ double squares(const T* p, uint64_t left) {
+    double s = 0.0;
+    float x[kLane];
+    if (left >= kNormUnit &&
+        reinterpret_cast<uintptr_t>(p) % (kLane * sizeof(T)) == 0) {
+        load8(p + threadIdx.x * kLane, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane; j++) {
+            const uint32_t at = threadIdx.x + kThreads * j;
+            x[j] = at < left ? to_f(p[at]) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; j++) s += double(x[j]) * double(x[j]);
+    return s;
+}
+
+__device__ __forceinline__ double block_sum(double s) {
+    __shared__ double red[kWarps];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = s;
+    __syncthreads();
+    s = 0.0;
+    for (int k = 0; k < kWarps; k++) s += red[k];
+    return s;
+}
+
+__global__ void __launch_bounds__(kThreads)
+        k_norm_parts(const __grid_constant__ NormTable t, double* part,
+                     int add) {
+    const uint64_t all = t.first[t.count];
+    const uint32_t end = uint32_t(all * (blockIdx.x + 1) / gridDim.x);
+    double s = 0.0;
+    uint32_t ti = kNone;
+    for (uint32_t b = uint32_t(all * blockIdx.x / gridDim.x); b < end; b++) {
+        if (ti == kNone) ti = tensor_of(t, b);
+        while (b >= t.first[ti + 1]) ti++;
+        const uint64_t at = uint64_t(b - t.first[ti]) * kNormUnit;
+        const uint64_t left = t.n[ti] - at;
+        if (t.type[ti] == 0)
+            s += squares(static_cast<const float*>(t.p[ti]) + at, left);
+        else if (t.type[ti] == 1)
+            s += squares(static_cast<const __half*>(t.p[ti]) + at, left);
+        else
+            s += squares(static_cast<const __nv_bfloat16*>(t.p[ti]) + at,
+                         left);
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0)
+        part[blockIdx.x] = add ? part[blockIdx.x] + s : s;
+}
+
+__global__ void __launch_bounds__(kThreads)
+        k_norm_finish(const double* part, int n, float* out) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += kThreads) s += part[i];
+    s = block_sum(s);
+    if (threadIdx.x == 0) out[0] = float(sqrt(s));
+}
+
+}  // namespace
+
+void adamw_op(const AdamWArgs& a, cudaStream_t s) {
+    if (a.n_tensors == 0) return;
+    AdamWHyper h{};
+    h.b1 = float(a.beta1);
+    h.omb1 = float(1.0 - a.beta1);
+    h.b2 = float(a.beta2);
+    h.omb2 = float(1.0 - a.beta2);
+    h.eps = float(a.eps);
+    h.ln_b1 = float(std::log(a.beta1));
+    h.ln_b2 = float(std::log(a.beta2));
+    h.lo = a.clamp_lo;
+    h.hi = a.clamp_hi;
+    h.max_norm = float(a.max_norm);
+    h.lr = a.lr;
+    h.wd = a.weight_decay;
+    h.lr_device = a.lr_device;
+    h.norm = a.max_norm > 0.0 ? a.grad_norm : nullptr;
+    h.seed = a.seed;
+    h.ticket = a.ticket;
+    ProfScope ps("adamw", s);
+    auto by_bits = [&](auto t) {
+        using T = decltype(t);
+        if (a.state_bits == 8) adamw_t<T, 8>(a, h, s);
+        else adamw_t<T, 32>(a, h, s);
+    };
+    if (a.dtype == 0) by_bits(float());
+    else if (a.dtype == 1) by_bits(__half());
+    else by_bits(__nv_bfloat16());
+}
+
+size_t grad_norm_workspace() { return kNormMost * sizeof(double); }
+
+void grad_norm_op(uint32_t n_tensors, const void* const* tensors,
+                  const uint64_t* numel, const int32_t* dtypes, float* out,
+                  void* workspace, cudaStream_t s) {
+    double* part = static_cast<double*>(workspace);
+    auto units = [&](uint32_t i) {
+        return (numel[i] + kNormUnit - 1) / kNormUnit;
+    };
+    uint64_t all = 0;
+    for (uint32_t i = 0; i < n_tensors; i++) all += units(i);
+    const int grid = int(std::max<uint64_t>(
+            1, std::min<uint64_t>(
+                       all, std::min(kNormMost, sm_count() * kNormCtasPerSm))));
+    ProfScope ps("grad_norm", s);
+    uint32_t i = 0;
+    int add = 0;
+    do {
+        NormTable t;
+        uint64_t blocks = 0;
+        uint32_t k = 0;
+        for (; i < n_tensors && k < kNormCap; i++, k++) {
+            if (k > 0 && blocks + units(i) > kMostBlocks) break;
+            t.p[k] = tensors[i];
+            t.n[k] = numel[i];
+            t.type[k] = uint8_t(dtypes[i]);
+            t.first[k] = uint32_t(blocks);
+            blocks += units(i);
+        }
+        t.first[k] = uint32_t(blocks);
+        t.count = k;
+        k_norm_parts<<<grid, kThreads, 0, s>>>(t, part, add);
+        DRESSI_CUDA(cudaGetLastError());
+        add = 1;
+    } while (i < n_tensors);
+    k_norm_finish<<<1, kThreads, 0, s>>>(part, grid, out);
+    DRESSI_CUDA(cudaGetLastError());
+}
+
+}  // namespace dressi

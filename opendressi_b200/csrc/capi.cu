@@ -1052,6 +1052,217 @@ int dressi_regularized_grad(const float* pos, uint32_t n_verts,
     });
 }
 
+// ------------------------------------------------------ learning operators
+
+namespace {
+
+bool aligned_to(const void* p, size_t a) {
+    return reinterpret_cast<uintptr_t>(p) % a == 0;
+}
+
+size_t dtype_bytes(int32_t t) { return t == DRESSI_F32 ? 4 : 2; }
+
+void dtype_check(int32_t t) {
+    DRESSI_REQUIRE(t == DRESSI_F32 || t == DRESSI_F16 || t == DRESSI_BF16,
+                   "dtype must be DRESSI_F32, DRESSI_F16 or DRESSI_BF16");
+}
+
+GroupNormArgs group_norm_args(const dressi_group_norm_desc* d) {
+    DRESSI_REQUIRE(d, "null pointer");
+    DRESSI_REQUIRE(d->struct_size == sizeof(dressi_group_norm_desc),
+                   "group_norm: struct_size mismatch");
+    dtype_check(d->dtype);
+    DRESSI_REQUIRE(d->activation >= DRESSI_ACT_NONE &&
+                           d->activation <= DRESSI_ACT_SILU,
+                   "group_norm: unknown activation");
+    DRESSI_REQUIRE(d->channels >= 1 && d->channels <= (1u << 24),
+                   "group_norm: 1 to 2^24 channels");
+    DRESSI_REQUIRE(d->groups >= 1 && d->channels % d->groups == 0,
+                   "group_norm: groups must divide channels");
+    DRESSI_REQUIRE(std::isfinite(d->eps) && d->eps >= 0.f,
+                   "group_norm: eps must be finite and not negative");
+    DRESSI_REQUIRE(d->rows < (1ull << 36) && d->n < (1ull << 36) &&
+                           (d->n == 0 || d->rows == 0 ||
+                            d->n * double(d->rows) * d->channels < 0x1p48),
+                   "group_norm: too many values");
+    GroupNormArgs a{};
+    a.n = d->n;
+    a.rows = d->rows;
+    a.C = int(d->channels);
+    a.G = int(d->groups);
+    a.eps = d->eps;
+    a.act = d->activation;
+    a.dtype = d->dtype;
+    return a;
+}
+
+void group_norm_space(const GroupNormArgs& a, bool grad, const void* workspace,
+                      size_t bytes) {
+    DRESSI_REQUIRE(workspace && aligned_to(workspace, 16),
+                   "group_norm: the workspace must be aligned to 16 bytes");
+    DRESSI_REQUIRE(bytes >= group_norm_workspace(a, grad),
+                   "group_norm: workspace too small");
+}
+
+}  // namespace
+
+int dressi_group_norm_workspace(const dressi_group_norm_desc* d, int grad,
+                                size_t* bytes) {
+    return guarded([&] {
+        DRESSI_REQUIRE(bytes, "null pointer");
+        *bytes = group_norm_workspace(group_norm_args(d), grad != 0);
+    });
+}
+
+int dressi_group_norm(const dressi_group_norm_desc* d, const void* x,
+                      const float* weight, const float* bias, void* y,
+                      float* mean, float* rstd, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const GroupNormArgs a = group_norm_args(d);
+        if (a.n == 0 || a.rows == 0) return;
+        DRESSI_REQUIRE(x && y, "null pointer");
+        DRESSI_REQUIRE((mean == nullptr) == (rstd == nullptr),
+                       "group_norm: mean and rstd, or neither");
+        DRESSI_REQUIRE(aligned_to(x, dtype_bytes(a.dtype)) &&
+                               aligned_to(y, dtype_bytes(a.dtype)),
+                       "group_norm: image not aligned to its element");
+        group_norm_space(a, false, workspace, workspace_bytes);
+        group_norm_op(a, x, weight, bias, y, mean, rstd, workspace,
+                      as_stream(stream));
+    });
+}
+
+int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
+                           const void* x, const float* weight,
+                           const float* bias, const float* mean,
+                           const float* rstd, void* dx, float* dweight,
+                           float* dbias, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const GroupNormArgs a = group_norm_args(d);
+        const size_t es = dtype_bytes(a.dtype);
+        if (a.n != 0 && a.rows != 0) {
+            DRESSI_REQUIRE(dy && x && mean && rstd, "null pointer");
+            DRESSI_REQUIRE(aligned_to(dy, es) && aligned_to(x, es) &&
+                                   aligned_to(dx, es),
+                           "group_norm: image not aligned to its element");
+            group_norm_space(a, true, workspace, workspace_bytes);
+        }
+        if (!dx && !dweight && !dbias) return;
+        group_norm_grad_op(a, dy, x, weight, bias, mean, rstd, dx, dweight,
+                           dbias, workspace, as_stream(stream));
+    });
+}
+
+int dressi_grad_norm_workspace(size_t* bytes) {
+    return guarded([&] {
+        DRESSI_REQUIRE(bytes, "null pointer");
+        *bytes = grad_norm_workspace();
+    });
+}
+
+int dressi_grad_norm(uint32_t n_tensors, const void* const* tensors,
+                     const uint64_t* numel, const int32_t* dtypes, float* out,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        DRESSI_REQUIRE(out && workspace &&
+                               (n_tensors == 0 || (tensors && numel && dtypes)),
+                       "null pointer");
+        DRESSI_REQUIRE(aligned_to(workspace, 8) &&
+                               workspace_bytes >= grad_norm_workspace(),
+                       "grad_norm: workspace too small or not aligned to 8 "
+                       "bytes");
+        for (uint32_t i = 0; i < n_tensors; i++) {
+            dtype_check(dtypes[i]);
+            DRESSI_REQUIRE(numel[i] < (1ull << 40), "grad_norm: too long");
+            DRESSI_REQUIRE(numel[i] == 0 ||
+                                   (tensors[i] &&
+                                    aligned_to(tensors[i],
+                                               dtype_bytes(dtypes[i]))),
+                           "grad_norm: null or misaligned tensor");
+        }
+        grad_norm_op(n_tensors, tensors, numel, dtypes, out, workspace,
+                     as_stream(stream));
+    });
+}
+
+int dressi_adamw_step(const dressi_adamw_desc* d, void* stream) {
+    return guarded([&] {
+        DRESSI_REQUIRE(d, "null pointer");
+        DRESSI_REQUIRE(d->struct_size == sizeof(dressi_adamw_desc),
+                       "adamw: struct_size mismatch");
+        dtype_check(d->dtype);
+        DRESSI_REQUIRE(d->state_bits == 32 || d->state_bits == 8,
+                       "adamw: state_bits must be 32 or 8");
+        if (d->n_tensors == 0) return;
+        const bool bits8 = d->state_bits == 8;
+        DRESSI_REQUIRE(d->numel && d->params && d->grads && d->exp_avg &&
+                               d->exp_avg_sq && d->steps && d->ticket &&
+                               (!bits8 ||
+                                (d->exp_avg_scale && d->exp_avg_sq_scale)),
+                       "null pointer");
+        DRESSI_REQUIRE(d->lr_device || (std::isfinite(d->lr) && d->lr >= 0.0),
+                       "adamw: lr must be finite and not negative");
+        DRESSI_REQUIRE(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 &&
+                               d->beta2 < 1.0,
+                       "adamw: betas must be in [0, 1)");
+        DRESSI_REQUIRE(std::isfinite(d->eps) && d->eps >= 0.0,
+                       "adamw: eps must be finite and not negative");
+        DRESSI_REQUIRE(std::isfinite(d->weight_decay) &&
+                               d->weight_decay >= 0.0,
+                       "adamw: weight_decay must be finite and not negative");
+        DRESSI_REQUIRE(std::isfinite(d->max_norm) && d->max_norm >= 0.0 &&
+                               (d->max_norm == 0.0 || d->grad_norm),
+                       "adamw: max_norm must be finite and not negative, and "
+                       "comes with grad_norm");
+        DRESSI_REQUIRE(d->clamp_lo <= d->clamp_hi,
+                       "adamw: clamp_lo above clamp_hi");
+        const size_t es = dtype_bytes(d->dtype);
+        for (uint32_t i = 0; i < d->n_tensors; i++) {
+            DRESSI_REQUIRE(d->numel[i] < (1ull << 39), "adamw: too long");
+            DRESSI_REQUIRE(d->steps[i], "adamw: null step counter");
+            if (d->numel[i] == 0) continue;
+            DRESSI_REQUIRE(d->params[i] && d->grads[i] && d->exp_avg[i] &&
+                                   d->exp_avg_sq[i] &&
+                                   (!bits8 || (d->exp_avg_scale[i] &&
+                                               d->exp_avg_sq_scale[i])),
+                           "adamw: null tensor");
+            DRESSI_REQUIRE(aligned_to(d->params[i], es) &&
+                                   aligned_to(d->grads[i], es) &&
+                                   (bits8 || (aligned_to(d->exp_avg[i], 4) &&
+                                              aligned_to(d->exp_avg_sq[i], 4))),
+                           "adamw: tensor not aligned to its element");
+        }
+        AdamWArgs a{};
+        a.n_tensors = d->n_tensors;
+        a.dtype = d->dtype;
+        a.state_bits = d->state_bits;
+        a.params = d->params;
+        a.grads = d->grads;
+        a.exp_avg = d->exp_avg;
+        a.avg_sq = d->exp_avg_sq;
+        a.exp_avg_scale = d->exp_avg_scale;
+        a.avg_sq_scale = d->exp_avg_sq_scale;
+        a.steps = d->steps;
+        a.numel = d->numel;
+        a.index = d->index;
+        a.lr = d->lr;
+        a.beta1 = d->beta1;
+        a.beta2 = d->beta2;
+        a.eps = d->eps;
+        a.weight_decay = d->weight_decay;
+        a.lr_device = d->lr_device;
+        a.clamp_lo = d->clamp_lo;
+        a.clamp_hi = d->clamp_hi;
+        a.max_norm = d->max_norm;
+        a.grad_norm = d->grad_norm;
+        a.seed = d->seed;
+        a.ticket = d->ticket;
+        adamw_op(a, as_stream(stream));
+    });
+}
+
 // ---------------------------------------------------- split-sum IBL ops
 
 namespace {

@@ -628,6 +628,56 @@ void interpolate_grad_op(const float* gy, int n_comp, int n_verts,
                          int n_faces, int views, int W, int H, float* grad,
                          uint32_t* status, cudaStream_t s);
 
+// --- group normalisation (group_norm.cu) ---
+struct GroupNormArgs {
+    uint64_t n, rows;  // x [n][rows][C]
+    int C, G;
+    float eps;
+    int act;    // 0 none, 1 relu, 2 silu
+    int dtype;  // 0 f32, 1 f16, 2 bf16
+};
+// Bytes of workspace that a forward (grad: backward) call needs.
+size_t group_norm_workspace(const GroupNormArgs& a, bool grad);
+// y = act(group_norm(x)); mean / rstd [n][G] are written where not null.
+void group_norm_op(const GroupNormArgs& a, const void* x, const float* weight,
+                   const float* bias, void* y, float* mean, float* rstd,
+                   void* workspace, cudaStream_t s);
+// dx, dweight, dbias: each may be null.
+void group_norm_grad_op(const GroupNormArgs& a, const void* dy, const void* x,
+                        const float* weight, const float* bias,
+                        const float* mean, const float* rstd, void* dx,
+                        float* dweight, float* dbias, void* workspace,
+                        cudaStream_t s);
+
+// --- AdamW over many tensors, norm over many tensors (adamw.cu) ---
+struct AdamWArgs {
+    uint32_t n_tensors;
+    int dtype;       // of parameters and gradients: 0 f32, 1 f16, 2 bf16
+    int state_bits;  // 32 or 8
+    void* const* params;
+    const void* const* grads;
+    void* const* exp_avg;  // f32, or e4m3 codes
+    void* const* avg_sq;   // f32 exp_avg_sq, or e4m3 codes of its root
+    float* const* exp_avg_scale;  // 8 bits: a scale per block of 256
+    float* const* avg_sq_scale;
+    int32_t* const* steps;
+    const uint64_t* numel;
+    const uint32_t* index;  // what the random bits know a tensor by
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* lr_device;  // null: lr
+    float clamp_lo, clamp_hi;
+    double max_norm;         // 0: no clipping
+    const float* grad_norm;  // device; with max_norm
+    uint32_t seed;
+    uint32_t* ticket;
+};
+void adamw_op(const AdamWArgs& a, cudaStream_t s);
+size_t grad_norm_workspace();
+// out[0] = sqrt(sum of squares over every tensor).
+void grad_norm_op(uint32_t n_tensors, const void* const* tensors,
+                  const uint64_t* numel, const int32_t* dtypes, float* out,
+                  void* workspace, cudaStream_t s);
+
 // --- image fitting (C1) ---
 struct FitBuffers {
     float* param;   // [n]

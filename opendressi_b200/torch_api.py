@@ -30,6 +30,12 @@ As in the reference:
 - ``rasterize_soft`` returns [N, K, H, W, 4] RasterizeSoft layers (K depth
   peels) and is differentiable w.r.t. pos through the dist channel.
 
+An extension, for networks that learn on rendered images:
+
+- ``group_norm`` normalises groups of channels of a channels-last image
+  [N, H, W, C] (float32, float16 or bfloat16) and applies an activation;
+  differentiable w.r.t. x, weight and bias.
+
 Clip positions are OpenGL-style (z in [-w, w]); they are converted to the
 Vulkan depth range (z_vk = 0.5 (z + w)) before rasterization and the
 gradients flow back through that conversion (convert.py:93-109).
@@ -39,17 +45,19 @@ from __future__ import annotations
 
 import threading
 import weakref
+from typing import Optional
 
 import numpy as np
 import torch
 from torch.library import custom_op
 
 from . import _native as N
+from . import ops
 from .ops import check_status, status_word
 
 __all__ = ["RasterizeContext", "RasterizeVulkanContext", "rasterize",
            "interpolate", "texture", "antialias", "rasterize_soft",
-           "check_status"]
+           "group_norm", "check_status"]
 
 Tensor = torch.Tensor
 
@@ -645,3 +653,110 @@ def rasterize_soft(ctx: RasterizeContext, pos, tri, resolution,
     return _rasterize_soft_op(_clip_gl_to_vk(pos_b), md.faces_f, md.faces_seq,
                               md.corner_face_id, h, w, float(radius_px),
                               max(1, int(peels)))
+
+
+# --------------------------------------------------- custom ops: group_norm
+
+@custom_op("dressi_b200::group_norm", mutates_args=())
+def _group_norm_op(x: Tensor, weight: Optional[Tensor],
+                   bias: Optional[Tensor], num_groups: int, eps: float,
+                   activation: str) -> tuple[Tensor, Tensor, Tensor]:
+    return ops.group_norm(x, num_groups, weight, bias, eps, activation, True)
+
+
+@_group_norm_op.register_fake
+def _(x, weight, bias, num_groups, eps, activation):
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean = x.new_empty((x.shape[0], num_groups), dtype=torch.float32)
+    return y, mean, torch.empty_like(mean)
+
+
+@custom_op("dressi_b200::group_norm_grad", mutates_args=())
+def _group_norm_grad_op(dy: Tensor, x: Tensor, weight: Optional[Tensor],
+                        bias: Optional[Tensor], mean: Tensor, rstd: Tensor,
+                        num_groups: int, eps: float, activation: str
+                        ) -> tuple[Tensor, Tensor, Tensor]:
+    dx, dw, db = ops.group_norm_grad(dy, x, num_groups, weight, bias, mean,
+                                     rstd, eps, activation)
+    empty = mean.new_empty((0,))
+    return (dx, empty if dw is None else dw,
+            torch.empty_like(empty) if db is None else db)
+
+
+@_group_norm_grad_op.register_fake
+def _(dy, x, weight, bias, mean, rstd, num_groups, eps, activation):
+    c = x.shape[-1]
+    return (torch.empty_like(x, memory_format=torch.contiguous_format),
+            mean.new_empty((0 if weight is None else c,)),
+            mean.new_empty((0 if bias is None else c,)))
+
+
+def _gn_setup(ctx, inputs, output):
+    x, weight, bias, num_groups, eps, activation = inputs
+    _, mean, rstd = output
+    ctx.save_for_backward(x, weight, bias, mean, rstd)
+    ctx.meta = (num_groups, eps, activation)
+    ctx.mark_non_differentiable(mean, rstd)
+
+
+def _gn_backward(ctx, g, _gm, _gr):
+    x, weight, bias, mean, rstd = ctx.saved_tensors
+    dx, dw, db = _group_norm_grad_op(g, x, weight, bias, mean, rstd,
+                                     *ctx.meta)
+    return (dx, None if weight is None else dw, None if bias is None else db,
+            None, None, None)
+
+
+_group_norm_op.register_autograd(_gn_backward, setup_context=_gn_setup)
+
+
+class _GroupNorm(torch.autograd.Function):
+    """The op outside of a trace: the custom op's Python layers cost more
+    than a small image's kernels do."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, num_groups, eps, activation):
+        x = x if x.is_contiguous() else x.contiguous()
+        y, mean, rstd = ops.group_norm(x, num_groups, weight, bias, eps,
+                                       activation, True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.meta = (num_groups, eps, activation)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        num_groups, eps, activation = ctx.meta
+        return (*ops.group_norm_grad(g, x, num_groups, weight, bias, mean,
+                                     rstd, eps, activation,
+                                     ctx.needs_input_grad[:3]),
+                None, None, None)
+
+
+def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
+               activation: str = "none"):
+    """act(group_norm(x)) of a channels-last image or table x [N, ..., C].
+
+    Each sample's num_groups groups of C / num_groups neighbouring channels
+    are brought to mean 0 and (biased) variance 1 over all pixels, scaled and
+    shifted by weight and bias [C] (or not) and passed through the activation
+    ("none", "relu" or "silu"). x is float32, float16 or bfloat16 and so is
+    the result; statistics are taken in 32 bits and more. A channels-last
+    tensor of shape [N, C, H, W] is given as x.permute(0, 2, 3, 1), which
+    copies nothing. Differentiable once, w.r.t. x, weight and bias."""
+    weight = None if weight is None else _f32_table(weight, "weight")
+    bias = None if bias is None else _f32_table(bias, "bias")
+    if torch.compiler.is_compiling():
+        return _group_norm_op(x, weight, bias, num_groups, float(eps),
+                              activation)[0]
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNorm.apply(x, weight, bias, num_groups, eps, activation)
+    return ops.group_norm(x, num_groups, weight, bias, eps, activation)
+
+
+def _f32_table(t, name):
+    if not isinstance(t, Tensor) or not t.is_cuda:
+        raise N.DressiError(N.ERR_INVALID, f"{name} must be a CUDA tensor")
+    return t if t.dtype == torch.float32 else t.to(torch.float32)
