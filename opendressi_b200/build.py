@@ -1,4 +1,5 @@
-"""Builds libdressi_b200.so in-tree with nvcc for sm_100a.
+"""Builds libdressi_b200.so in-tree with nvcc for sm_100a, and the torch
+binding of its learning operators (_torch_binding.so) with g++.
 
     python -m opendressi_b200.build        # or opendressi_b200.build.build()
 
@@ -19,6 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdressi_b200.so")
+BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
+BINDING = os.path.join(HERE, "_torch_binding.so")
 SOURCES = ["capi.cu", "soft_raster.cu", "silhouette.cu", "hard_raster.cu",
            "fit.cu", "noalloc.cu",
            "antialias.cu", "texture.cu", "interp.cu", "regularize.cu",
@@ -64,20 +67,64 @@ def nvcc() -> str:
     return cand if os.path.exists(cand) else "nvcc"
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB):
+def _older(target: str, deps: list[str]) -> bool:
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(ROOT, "include", "dressi_b200.h"))
-    deps.append(os.path.abspath(__file__))
+    t = os.path.getmtime(target)
+    deps = deps + [os.path.join(ROOT, "include", "dressi_b200.h"),
+                   os.path.abspath(__file__)]
     return any(os.path.getmtime(p) > t for p in deps if os.path.exists(p))
 
 
+def _stale() -> bool:
+    return _older(LIB, [os.path.join(CSRC, f) for f in SOURCES + HEADERS])
+
+
+def _binding_command() -> list[str]:
+    """g++ for the torch binding: an extension module over torch's headers
+    and libdressi_b200.so (found beside it)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    lib = cpp_extension.library_paths()
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+            "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_torch_binding",
+            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+            *[f"-isystem{p}" for p in cpp_extension.include_paths()],
+            f"-isystem{os.path.join(cuda, 'include')}",
+            f"-isystem{sysconfig.get_paths()['include']}", BINDING_SOURCE,
+            "-o", BINDING, *[f"-L{p}" for p in lib], f"-L{HERE}",
+            "-l:libdressi_b200.so", "-Wl,-rpath,$ORIGIN", "-lc10",
+            "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+            "-ltorch_python"]
+
+
+def _build_binding(force: bool, verbose: bool) -> None:
+    if not force and not _older(BINDING, [BINDING_SOURCE]):
+        return
+    cmd = _binding_command()
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    out = subprocess.run(cmd, capture_output=True, text=True)
+    if out.returncode != 0:
+        raise RuntimeError("g++ failed on torch_binding.cpp:\n" + out.stdout +
+                           out.stderr)
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int = 8) -> str:
-    """Compiles every translation unit and links the shared library."""
+    """Compiles every translation unit, links the shared library and the
+    torch binding over it."""
+    _build_library(force, verbose, jobs)
+    _build_binding(force, verbose)
+    return LIB
+
+
+def _build_library(force: bool, verbose: bool, jobs: int) -> None:
     if not force and not _stale():
-        return LIB
+        return
     obj_dir = os.path.join(HERE, "_build")
     os.makedirs(obj_dir, exist_ok=True)
     objs, procs = [], []
@@ -99,7 +146,6 @@ def build(force: bool = False, verbose: bool = False, jobs: int = 8) -> str:
     out = subprocess.run(link, capture_output=True, text=True)
     if out.returncode != 0:
         raise RuntimeError("link failed:\n" + out.stdout + out.stderr)
-    return LIB
 
 
 def _wait(item):

@@ -10,9 +10,6 @@ device status word -- out-of-range indices) raise DressiError here.
 
 from __future__ import annotations
 
-import ctypes as C
-from array import array
-
 import torch
 
 from . import _native as N
@@ -721,103 +718,14 @@ def face_fetch_grad(gy, idx, prj0, prj1, prj2, seed: float = 0.0,
 
 # ------------------------------------------------------ learning operators
 
-_DTYPES = {torch.float32: N.F32, torch.float16: N.F16,
-           torch.bfloat16: N.BF16}
-ACTIVATIONS = {"none": N.ACT_NONE, "relu": N.ACT_RELU, "silu": N.ACT_SILU}
-
-
-class _On:
-    """Makes a tensor's device current for a call."""
-
-    __slots__ = ("dev", "prev")
-
-    def __init__(self, t):
-        self.dev = t.device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
-
-
-def _stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _typed(t, name: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise N.DressiError(N.ERR_INVALID, f"{name} must be a CUDA tensor")
-    if t.dtype not in _DTYPES:
-        raise N.DressiError(N.ERR_INVALID, f"{name} must be float32, float16 "
-                            f"or bfloat16, got {t.dtype}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _channel_table(t, name: str, x: torch.Tensor):
-    if t is None:
-        return None
-    t = _dev(t, name)
-    if t.shape != (x.shape[-1],) or t.device != x.device:
-        raise N.DressiError(N.ERR_INVALID, f"{name} must be [{x.shape[-1]}] "
-                            f"on {x.device}, got {tuple(t.shape)} on "
-                            f"{t.device}")
-    return t
-
-
-def _group_norm_desc(x, num_groups, eps, activation) -> N.GroupNormDesc:
-    if x.dim() < 2:
-        raise N.DressiError(N.ERR_INVALID, "x must be [N, ..., C], got "
-                            f"{tuple(x.shape)}")
-    if activation not in ACTIVATIONS:
-        raise N.DressiError(N.ERR_INVALID, "activation must be one of "
-                            f"{list(ACTIVATIONS)}, got {activation!r}")
-    n, c = x.shape[0], x.shape[-1]
-    num_groups = int(num_groups)
-    if c < 1 or num_groups < 1 or c % num_groups:
-        raise N.DressiError(N.ERR_INVALID, f"{num_groups} groups do not "
-                            f"divide {c} channels")
-    rows = 1
-    for k in x.shape[1:-1]:
-        rows *= k
-    return N.GroupNormDesc(C.sizeof(N.GroupNormDesc), _DTYPES[x.dtype],
-                           ACTIVATIONS[activation], c, num_groups,
-                           float(eps), n, rows)
-
-
-def _group_norm_space(d, grad: bool, x) -> torch.Tensor:
-    size = C.c_size_t()
-    N.call("dressi_group_norm_workspace", d, int(grad), size)
-    return torch.empty(size.value, dtype=torch.uint8, device=x.device)
-
-
 def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
                activation: str = "none", stats: bool = False):
     """act(group_norm(x)) of a channels-last x [N, ..., C] in float32,
-    float16 or bfloat16; weight, bias [C] float32 or None. With `stats` also
-    the mean and 1 / deviation [N, num_groups] that group_norm_grad takes."""
-    x = _typed(x, "x")
-    d = _group_norm_desc(x, num_groups, eps, activation)
-    weight = _channel_table(weight, "weight", x)
-    bias = _channel_table(bias, "bias", x)
-    y = torch.empty_like(x)
-    mean = rstd = None
-    if stats:
-        mean = torch.empty((x.shape[0], int(num_groups)), dtype=torch.float32,
-                           device=x.device)
-        rstd = torch.empty_like(mean)
-    if x.numel():
-        with _On(x):
-            space = _group_norm_space(d, False, x)
-            N.call("dressi_group_norm", d, x.data_ptr(), _ptr(weight),
-                   _ptr(bias), y.data_ptr(), _ptr(mean), _ptr(rstd),
-                   space.data_ptr(), space.numel(), _stream_of(x))
-    elif stats:  # a sample without pixels
-        mean.zero_()
-        rstd.zero_()
+    float16 or bfloat16; weight, bias [C] float32 or None; activation "none",
+    "relu" or "silu". With `stats` also the mean and 1 / deviation
+    [N, num_groups] that group_norm_grad takes."""
+    y, mean, rstd = binding().group_norm_forward(
+        x, num_groups, weight, bias, eps, activation, stats)
     return (y, mean, rstd) if stats else y
 
 
@@ -826,33 +734,8 @@ def group_norm_grad(dy, x, num_groups: int, weight, bias, mean, rstd,
                     want=(True, True, True)):
     """(dx, dweight, dbias) of group_norm for dy, from x and its statistics;
     None where `want` says so or where weight / bias is None."""
-    x = _typed(x, "x")
-    dy = _typed(dy, "dy")
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
-        raise N.DressiError(N.ERR_INVALID, "dy must be like x")
-    d = _group_norm_desc(x, num_groups, eps, activation)
-    weight = _channel_table(weight, "weight", x)
-    bias = _channel_table(bias, "bias", x)
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if (_dev(t, name).shape != (x.shape[0], int(num_groups))
-                or t.device != x.device):
-            raise N.DressiError(N.ERR_INVALID, f"{name} must be [N, groups] "
-                                f"on {x.device}, got {tuple(t.shape)} on "
-                                f"{t.device}")
-    mean, rstd = mean.contiguous(), rstd.contiguous()
-    c = x.shape[-1]
-    dx = torch.empty_like(x) if want[0] else None
-    dw = (torch.empty(c, dtype=torch.float32, device=x.device)
-          if want[1] and weight is not None else None)
-    db = (torch.empty(c, dtype=torch.float32, device=x.device)
-          if want[2] and bias is not None else None)
-    with _On(x):
-        space = _group_norm_space(d, True, x)
-        N.call("dressi_group_norm_grad", d, dy.data_ptr(), x.data_ptr(),
-               _ptr(weight), _ptr(bias), mean.data_ptr(), rstd.data_ptr(),
-               _ptr(dx), _ptr(dw), _ptr(db), space.data_ptr(), space.numel(),
-               _stream_of(x))
-    return dx, dw, db
+    return tuple(binding().group_norm_backward(
+        dy, x, num_groups, weight, bias, mean, rstd, eps, activation, *want))
 
 
 def grad_norm(tensors, out=None) -> torch.Tensor:
@@ -861,24 +744,23 @@ def grad_norm(tensors, out=None) -> torch.Tensor:
     summed in 64 bits in an order that the sizes alone give."""
     if isinstance(tensors, torch.Tensor):
         tensors = [tensors]
-    tensors = [_typed(t, "tensor") for t in tensors]
-    dev = tensors[0].device if tensors else torch.device(
-        "cuda", torch.cuda.current_device())
-    if any(t.device != dev for t in tensors):
-        raise N.DressiError(N.ERR_INVALID, "tensors on several devices")
-    if out is None:
-        out = torch.empty((), dtype=torch.float32, device=dev)
-    elif out.dtype != torch.float32 or out.numel() != 1 or out.device != dev:
-        raise N.DressiError(N.ERR_INVALID, "out must hold one float32 on "
-                            f"{dev}")
-    ptrs = array("Q", [t.data_ptr() for t in tensors])
-    sizes = array("Q", [t.numel() for t in tensors])
-    types = array("i", [_DTYPES[t.dtype] for t in tensors])
-    size = C.c_size_t()
-    N.call("dressi_grad_norm_workspace", size)
-    with _On(out):
-        space = torch.empty(size.value, dtype=torch.uint8, device=dev)
-        N.call("dressi_grad_norm", len(tensors), ptrs.buffer_info()[0],
-               sizes.buffer_info()[0], types.buffer_info()[0], out.data_ptr(),
-               space.data_ptr(), space.numel(), _stream_of(out))
-    return out
+    return binding().grad_norm(list(tensors), out)
+
+
+_binding = None
+
+
+def binding():
+    """The learning operators' binding (csrc/torch_binding.cpp)."""
+    global _binding
+    if _binding is None:
+        N.load()
+        try:
+            from . import _torch_binding
+        except ImportError as e:
+            raise N.DressiError(
+                N.ERR_INVALID, f"_torch_binding.so does not load ({e}): build "
+                "it with `python -m opendressi_b200.build` (there is no "
+                "fallback implementation)") from e
+        _binding = _torch_binding
+    return _binding

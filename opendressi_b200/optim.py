@@ -9,36 +9,17 @@ counters on the device, so it can be captured in a CUDA graph.
 
 from __future__ import annotations
 
-import ctypes as C
 import math
-from array import array
 
 import torch
 
 from . import _native as N
-from .ops import _DTYPES, _On, _stream_of, grad_norm
+from .ops import binding, grad_norm
 
 __all__ = ["AdamW", "grad_norm"]
 
 _BLOCK = 256  # values of 8-bit state that share a scale
-
-
-def _dense(t: torch.Tensor) -> bool:
-    """Whether t's values fill its extent in memory, in some order, once."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted(zip(t.stride(), t.shape)):
-        if size != 1:
-            if stride != want:
-                return False
-            want *= size
-    return True
-
-
-def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return (a.is_contiguous() and b.is_contiguous()) or \
-        a.stride() == b.stride()
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 class _Pack:
@@ -46,64 +27,45 @@ class _Pack:
     parameter at a multiple of 256 values of it."""
 
     def __init__(self, params, state_bits: int, index: int):
-        dev = params[0].device if params else None
         self.params = params
-        self.numel = [p.numel() for p in params]
-        self.dtype = [p.dtype for p in params]
-        self.stride = [p.stride() for p in params]
-        blocks = [-(-n // _BLOCK) for n in self.numel]
-        first = [0]
-        for b in blocks:
-            first.append(first[-1] + b)
-        total = first[-1]
         self.flat = {}
-        if params:
-            wide = dict(dtype=torch.float32, device=dev)
-            code = dict(dtype=torch.float8_e4m3fn, device=dev)
-            self.flat["step"] = torch.zeros(len(params), dtype=torch.int32,
-                                            device=dev)
-            if state_bits == 32:
-                self.flat["exp_avg"] = torch.zeros(total * _BLOCK, **wide)
-                self.flat["exp_avg_sq"] = torch.zeros(total * _BLOCK, **wide)
-            else:
-                for k in ("exp_avg", "root_avg_sq"):
-                    self.flat[k] = torch.zeros(total * _BLOCK, **code)
-                    self.flat[k + "_scale"] = torch.zeros(total, **wide)
         self.views = []
+        self.rows = None
+        if not params:
+            return
+        first = [0]
+        for p in params:
+            first.append(first[-1] - (-p.numel() // _BLOCK))
+        total = first[-1]
+        dev = params[0].device
+        wide = dict(dtype=torch.float32, device=dev)
+        code = dict(dtype=torch.float8_e4m3fn, device=dev)
+        flat = {"step": torch.zeros(len(params), dtype=torch.int32,
+                                    device=dev)}
+        if state_bits == 32:
+            kinds = ("exp_avg", "exp_avg_sq")
+            for k in kinds:
+                flat[k] = torch.zeros(total * _BLOCK, **wide)
+        else:
+            kinds = ("exp_avg", "root_avg_sq")
+            for k in kinds:
+                flat[k] = torch.zeros(total * _BLOCK, **code)
+                flat[k + "_scale"] = torch.zeros(total, **wide)
         for i, p in enumerate(params):
             view = {}
-            for k, flat in self.flat.items():
+            for k, t in flat.items():
                 if k == "step":
-                    view[k] = flat[i]
+                    view[k] = t[i]
                 elif k.endswith("_scale"):
-                    view[k] = flat[first[i]:first[i + 1]]
+                    view[k] = t[first[i]:first[i + 1]]
                 else:  # in the parameter's own order of memory
-                    view[k] = flat.as_strided(p.shape, p.stride(),
-                                              first[i] * _BLOCK)
+                    view[k] = t.as_strided(p.shape, p.stride(),
+                                           first[i] * _BLOCK)
             self.views.append(view)
-        second = "exp_avg_sq" if state_bits == 32 else "root_avg_sq"
-        size = 4 if state_bits == 32 else 1
-
-        def at(kind, step):
-            if kind not in self.flat:
-                return [0] * len(params)
-            base = self.flat[kind].data_ptr()
-            return [base + f * step for f in first[:-1]]
-
-        steps = self.flat["step"].data_ptr() if params else 0
-        # what each parameter's state is called by in the C call
-        self.rows = list(zip(
-            self.numel, at("exp_avg", _BLOCK * size),
-            at(second, _BLOCK * size), at("exp_avg_scale", 4),
-            at(second + "_scale", 4),
-            [steps + 4 * i for i in range(len(params))],
-            range(index, index + len(params))))
-        self.whole = self.columns(range(len(params)))
-
-    def columns(self, which):
-        """The C call's host arrays for the parameters `which`."""
-        cols = list(zip(*(self.rows[i] for i in which))) or [()] * 7
-        return [array("Q", c) for c in cols[:6]] + [array("I", cols[6])]
+        self.flat = flat
+        self.rows = binding().Pack(
+            params, first[:-1], flat["step"], *(flat[k] for k in kinds),
+            *(flat.get(k + "_scale") for k in kinds), index, state_bits)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -199,7 +161,7 @@ class AdamW(torch.optim.Optimizer):
             if p.device != dev:
                 raise N.DressiError(N.ERR_INVALID,
                                     "parameters on several devices")
-            if not _dense(p):
+            if p.layout != torch.strided or not binding().dense(p):
                 raise N.DressiError(N.ERR_INVALID, "a parameter's memory must "
                                     "be dense and not overlap itself")
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() *
@@ -231,26 +193,18 @@ class AdamW(torch.optim.Optimizer):
 
     # --------------------------------------------------------------- step
 
-    def _gradients(self, pack: _Pack) -> list:
-        """Each parameter's gradient in the parameter's order of memory."""
-        grads = []
-        for p, n, dtype, stride in zip(pack.params, pack.numel, pack.dtype,
-                                       pack.stride):
-            g = p.grad
-            if p.dtype is not dtype or p.numel() != n or \
-                    p.stride() != stride or p.device != self._device:
-                raise N.DressiError(N.ERR_INVALID, "a parameter changed its "
-                                    "type, shape or device; make a new "
-                                    "optimizer")
-            if g is not None:
-                if g.is_sparse or g.dtype is not dtype or \
-                        g.shape != p.shape or g.device != self._device:
-                    raise N.DressiError(N.ERR_INVALID, "a gradient must be "
-                                        "dense and like its parameter")
-                if not _same_order(g, p):
-                    g = torch.empty_like(p).copy_(g)
-            grads.append(g)
-        return grads
+    def _numbers(self, group) -> tuple:
+        """What a step takes from a group, as the binding wants it."""
+        self._check_options(group)
+        lr, lr_device = group["lr"], None
+        if isinstance(lr, torch.Tensor):
+            if lr.is_cuda and lr.device != self._device:
+                raise N.DressiError(N.ERR_INVALID, "lr is on another device "
+                                    "than the parameters")
+            lr, lr_device = (0.0, lr) if lr.is_cuda else (float(lr), None)
+        lo, hi = group["clamp"] or (-math.inf, math.inf)
+        return (lr, lr_device, *group["betas"], group["eps"],
+                group["weight_decay"], lo, hi)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -260,51 +214,16 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._device is None:
-            return loss
-        grads = [self._gradients(pack) for pack in self._packs]
-        with _On(self._ticket):
-            if self.max_norm is not None:
-                grad_norm([g for gs in grads for g in gs if g is not None],
-                          out=self.last_norm)
-            for group, pack, gs in zip(self.param_groups, self._packs, grads):
-                self._check_options(group)
-                for dtype in dict.fromkeys(pack.dtype):
-                    which = [i for i, g in enumerate(gs)
-                             if g is not None and pack.dtype[i] is dtype]
-                    if which:
-                        self._launch(group, pack, gs, which, dtype)
+        packs, numbers = [], []
+        for pack, group in zip(self._packs, self.param_groups):
+            if pack.rows is not None:
+                packs.append(pack.rows)
+                numbers.append(self._numbers(group))
+        if packs:
+            binding().adamw_step(packs, numbers, self.max_norm or 0.0,
+                                 self.last_norm if self.max_norm else None,
+                                 self.seed, self._ticket)
         return loss
-
-    def _launch(self, group, pack, grads, which, dtype) -> None:
-        whole = len(which) == len(pack.params)
-        numel, m, v, sm, sv, steps, index = (
-            pack.whole if whole else pack.columns(which))
-        ptrs = array("Q", [pack.params[i].data_ptr() for i in which])
-        gptrs = array("Q", [grads[i].data_ptr() for i in which])
-        lr = group["lr"]
-        lr_device = None
-        if isinstance(lr, torch.Tensor):
-            if lr.is_cuda:
-                if lr.device != self._device:
-                    raise N.DressiError(N.ERR_INVALID, "lr is on another "
-                                        "device than the parameters")
-                lr, lr_device = 0.0, lr.data_ptr()
-            else:
-                lr = float(lr)
-        lo, hi = group["clamp"] or (-math.inf, math.inf)
-        clip = self.max_norm is not None
-        d = N.AdamWDesc(
-            C.sizeof(N.AdamWDesc), len(which), _DTYPES[dtype],
-            self.state_bits, numel.buffer_info()[0], ptrs.buffer_info()[0],
-            gptrs.buffer_info()[0], m.buffer_info()[0], v.buffer_info()[0],
-            sm.buffer_info()[0], sv.buffer_info()[0], steps.buffer_info()[0],
-            index.buffer_info()[0], lr, *group["betas"], group["eps"],
-            group["weight_decay"], lr_device,
-            self.max_norm if clip else 0.0,
-            self.last_norm.data_ptr() if clip else None, lo, hi, self.seed,
-            self._ticket.data_ptr())
-        N.call("dressi_adamw_step", d, _stream_of(self._ticket))
 
     # ---------------------------------------------------------- save / load
 

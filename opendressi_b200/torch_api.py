@@ -710,30 +710,6 @@ def _gn_backward(ctx, g, _gm, _gr):
 _group_norm_op.register_autograd(_gn_backward, setup_context=_gn_setup)
 
 
-class _GroupNorm(torch.autograd.Function):
-    """The op outside of a trace: the custom op's Python layers cost more
-    than a small image's kernels do."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, eps, activation):
-        x = x if x.is_contiguous() else x.contiguous()
-        y, mean, rstd = ops.group_norm(x, num_groups, weight, bias, eps,
-                                       activation, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.meta = (num_groups, eps, activation)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        num_groups, eps, activation = ctx.meta
-        return (*ops.group_norm_grad(g, x, num_groups, weight, bias, mean,
-                                     rstd, eps, activation,
-                                     ctx.needs_input_grad[:3]),
-                None, None, None)
-
-
 def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
                activation: str = "none"):
     """act(group_norm(x)) of a channels-last image or table x [N, ..., C].
@@ -745,18 +721,11 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
     the result; statistics are taken in 32 bits and more. A channels-last
     tensor of shape [N, C, H, W] is given as x.permute(0, 2, 3, 1), which
     copies nothing. Differentiable once, w.r.t. x, weight and bias."""
-    weight = None if weight is None else _f32_table(weight, "weight")
-    bias = None if bias is None else _f32_table(bias, "bias")
     if torch.compiler.is_compiling():
+        weight = None if weight is None else weight.to(torch.float32)
+        bias = None if bias is None else bias.to(torch.float32)
         return _group_norm_op(x, weight, bias, num_groups, float(eps),
                               activation)[0]
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _GroupNorm.apply(x, weight, bias, num_groups, eps, activation)
-    return ops.group_norm(x, num_groups, weight, bias, eps, activation)
-
-
-def _f32_table(t, name):
-    if not isinstance(t, Tensor) or not t.is_cuda:
-        raise N.DressiError(N.ERR_INVALID, f"{name} must be a CUDA tensor")
-    return t if t.dtype == torch.float32 else t.to(torch.float32)
+    # outside of a trace the same calls with their autograd in C++
+    return ops.binding().group_norm(x, num_groups, weight, bias, eps,
+                                    activation)

@@ -423,7 +423,7 @@ def test_groups_clamps_and_missing_gradients(cuda):
     # nan is not hidden by a clamp
     maps[0].grad[0, 0, 0] = math.nan
     opt.step()
-    assert math.isnan(float(maps[0][0, 0, 0]))
+    assert math.isnan(float(maps[0].detach()[0, 0, 0]))
 
 
 def test_many_tensors_in_several_launches(cuda):
@@ -704,7 +704,7 @@ def test_a_decoder_on_rendered_features(cuda):
     z = z.reshape(2, 48, 48, 24) * d[2] + d[3]
     exact = (((z * torch.sigmoid(z)) @ d[4] - target.double()) ** 2).mean()
     exact.backward()
-    assert abs(float(loss) / float(exact) - 1) < 1e-4  # tf32 stays off
+    assert abs(float(loss.detach()) / float(exact.detach()) - 1) < 1e-4  # tf32 stays off
     for p, e in zip(leaves, d):
         # sums over 4608 pixels of 32-bit products, and the interpolation's
         # atomics: 1e-4 of the largest

@@ -439,3 +439,20 @@ def test_refusals(cuda):
     with pytest.raises(DressiError):
         ops.group_norm_grad(x, x, 3, None, None, mean[:1], rstd)
     assert np.isfinite(float(y.sum()))
+
+
+def test_differentiable_once(cuda):
+    """A second derivative is refused, not taken as zero."""
+    torch = _torch()
+    from opendressi_b200 import torch_api as dr
+
+    x, dy, w, b = make(31, (2, 4, 3, 8), torch.float32)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    y = dr.group_norm(x, 2, w, b, activation="silu")
+    plain = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    grads = torch.autograd.grad(y, (x, w, b), dy, create_graph=True)
+    for a, e in zip(grads, plain):
+        assert torch.equal(a, e)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(grads[0].sum(), x)
