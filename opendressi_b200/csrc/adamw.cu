@@ -51,6 +51,7 @@ constexpr uint64_t kMostBlocks = 1ull << 31;  // of one launch
 struct AdamWHyper {
     float b1, omb1, b2, omb2, eps, ln_b1, ln_b2;
     float lo, hi, max_norm;
+    bool clamped;
     double lr, wd;
     const float* lr_device;
     const float* norm;
@@ -217,14 +218,15 @@ __device__ __forceinline__ float top_of(const float* x, bool* finite) {
     return fmaxf(__uint_as_float(top), 0x1p-100f);
 }
 
-// a >= 0 up or down to a neighbouring e4m3 value, up with the probability of
+// a in [0, 448 (1 + 2^-22)] up or down to a neighbouring e4m3 value (448 at
+// most: what two roundings left above it is cut), up with the probability of
 // its place between the two: 16 random bits (and a half) are added below the
 // 3 bits of fraction that stay. Below 2^-6 the values are 2^-9 apart, as they
 // are in [2^-6, 2^-5): the sum with 2^-6 is rounded instead.
 __device__ __forceinline__ float round_e4m3(float a, uint32_t bits16) {
     const float lift = a < 0x1p-6f ? 0x1p-6f : 0.f;
     const uint32_t b = __float_as_uint(a + lift) + (bits16 << 4 | 8u);
-    return fminf(__uint_as_float(b & 0xfff00000u) - lift, 448.f);
+    return __uint_as_float(b & 0xfff00000u) - lift;
 }
 
 // The codes of a lane's values x; ROOT: of values that are not negative and
@@ -236,8 +238,8 @@ __device__ __forceinline__ uint2 encode(const float* x, float inv, bool finite,
     float a[kLane];
 #pragma unroll
     for (int j = 0; j < kLane; j++) {
-        a[j] = round_e4m3(fminf(fabsf(x[j]) * inv, 448.f),
-                          ROOT ? bits[j] >> 16 : bits[j] & 0xffffu);
+        a[j] = round_e4m3(fabsf(x[j]) * inv, ROOT ? bits[j] >> 16
+                                                  : bits[j] & 0xffffu);
         if (ROOT) {
             a[j] = x[j] > 0.f ? fmaxf(a[j], 0x1p-9f) : a[j];
         } else {
@@ -259,6 +261,22 @@ __device__ __forceinline__ uint2 encode(const float* x, float inv, bool finite,
     return make_uint2(w[0], w[1]);
 }
 
+// sqrt to 2^-23.
+__device__ __forceinline__ float sqrt_fast(float v) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+template <int BITS>
+struct StateOf {
+    using type = float;
+};
+template <>
+struct StateOf<8> {
+    using type = uint8_t;
+};
+
 // The tensor whose blocks block b is among.
 template <typename Table>
 __device__ __forceinline__ uint32_t tensor_of(const Table& t, uint32_t b) {
@@ -272,7 +290,7 @@ __device__ __forceinline__ uint32_t tensor_of(const Table& t, uint32_t b) {
 }
 
 template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
         k_adamw(const __grid_constant__ AdamWTable<CAP> t,
                 const __grid_constant__ AdamWHyper h) {
     const int lane = threadIdx.x & 31;
@@ -288,89 +306,103 @@ __global__ void __launch_bounds__(kThreads)
     const double lr = h.lr_device ? double(*h.lr_device) : h.lr;
     const float decay = float(1.0 - lr * h.wd);
 
-    uint32_t ti = kNone, key = 0;
-    float size = 0.f, root = 0.f;
-    for (; b < b_end; b += kWarps) {
-        if (ti == kNone || b >= t.first[ti + 1]) {
-            if (ti == kNone) ti = tensor_of(t, b);
-            while (b >= t.first[ti + 1]) ti++;
-            const int32_t step = *t.step[ti] + 1;
-            // 1 - b^t = -expm1(t ln b): exact to a few 2^-24, also where b^t
-            // is next to 1
-            size = float(lr / double(-expm1f(float(step) * h.ln_b1)));
-            root = 1.f / sqrtf(-expm1f(float(step) * h.ln_b2));
-            if (BITS == 8)
-                key = wang_hash(wang_hash(h.seed ^ wang_hash(uint32_t(step))) +
-                                t.index[ti]);
-        }
-        const uint64_t at = uint64_t(b - t.first[ti]) * kBlock;
-        const uint64_t left = t.n[ti] - at;
-        const bool wide = t.wide[ti] && left >= kBlock;
-        uint32_t mask = 0xffu;
-        if (!wide && left < kBlock) {
-            mask = 0u;
+    uint32_t ti = b < b_end ? tensor_of(t, b) : 0u;
+    while (b < b_end) {  // tensor after tensor
+        while (b >= t.first[ti + 1]) ti++;
+        const uint32_t first = t.first[ti];
+        const uint32_t stop = min(b_end, t.first[ti + 1]);
+        const int32_t step = *t.step[ti] + 1;
+        // 1 - b^t = -expm1(t ln b): exact to a few 2^-24, also where b^t is
+        // next to 1
+        const float size =
+                float(lr / double(-expm1f(float(step) * h.ln_b1)));
+        const float root = 1.f / sqrtf(-expm1f(float(step) * h.ln_b2));
+        const uint32_t key =
+                BITS == 8 ? wang_hash(wang_hash(h.seed ^
+                                                wang_hash(uint32_t(step))) +
+                                      t.index[ti])
+                          : 0u;
+        T* const p0 = static_cast<T*>(t.p[ti]);
+        const T* const g0 = static_cast<const T*>(t.g[ti]);
+        using State = typename StateOf<BITS>::type;
+        State* const m0 = static_cast<State*>(t.m[ti]);
+        State* const v0 = static_cast<State*>(t.v[ti]);
+        float* const sm = t.sm[ti];
+        float* const sv = t.sv[ti];
+        const uint64_t n = t.n[ti];
+        const bool aligned = t.wide[ti];
+        for (; b < stop; b += kWarps) {
+            const uint32_t q = b - first;
+            const uint64_t at = uint64_t(q) * kBlock;
+            const bool wide = aligned && n - at >= kBlock;
+            uint32_t mask = 0xffu;
+            if (!wide && n - at < kBlock) {
+                mask = 0u;
 #pragma unroll
-            for (int j = 0; j < kLane; j++)
-                mask |= uint32_t(lane + 32 * j < int(left)) << j;
-        }
-        T* pp = static_cast<T*>(t.p[ti]) + at;
-        float p[kLane], g[kLane], m[kLane], v[kLane];
-        load_lane(static_cast<const T*>(t.g[ti]) + at, wide, mask, lane, g);
-        load_lane(static_cast<const T*>(pp), wide, mask, lane, p);
-        if (BITS == 32) {
-            load_lane(static_cast<const float*>(t.m[ti]) + at, wide, mask,
-                      lane, m);
-            load_lane(static_cast<const float*>(t.v[ti]) + at, wide, mask,
-                      lane, v);
-        } else {
-            const uint32_t q = b - t.first[ti];
-            const uint2 cm = load_codes(
-                    static_cast<const uint8_t*>(t.m[ti]) + at, wide, mask,
-                    lane);
-            const uint2 cv = load_codes(
-                    static_cast<const uint8_t*>(t.v[ti]) + at, wide, mask,
-                    lane);
-            const float sm = t.sm[ti][q], sv = t.sv[ti][q];
-            decode(cm, m);
-            decode(cv, v);
+                for (int j = 0; j < kLane; j++)
+                    mask |= uint32_t(lane + 32 * j < int(n - at)) << j;
+            }
+            float p[kLane], g[kLane], m[kLane], v[kLane];
+            load_lane(g0 + at, wide, mask, lane, g);
+            load_lane(static_cast<const T*>(p0 + at), wide, mask, lane, p);
+            if constexpr (BITS == 32) {
+                load_lane(static_cast<const float*>(m0 + at), wide, mask, lane,
+                          m);
+                load_lane(static_cast<const float*>(v0 + at), wide, mask, lane,
+                          v);
+            } else {
+                const uint2 cm = load_codes(m0 + at, wide, mask, lane);
+                const uint2 cv = load_codes(v0 + at, wide, mask, lane);
+                const float am = sm[q], av = sv[q];
+                decode(cm, m);
+                decode(cv, v);
+#pragma unroll
+                for (int j = 0; j < kLane; j++) {
+                    m[j] = m[j] * am;
+                    v[j] = v[j] * av;
+                    v[j] = v[j] * v[j];
+                }
+            }
 #pragma unroll
             for (int j = 0; j < kLane; j++) {
-                m[j] = m[j] * sm;
-                v[j] = v[j] * sv;
-                v[j] = v[j] * v[j];
+                const float gj = g[j] * scale;
+                m[j] = m[j] * h.b1 + gj * h.omb1;
+                v[j] = v[j] * h.b2 + (gj * gj) * h.omb2;
+                // the codes want the root as IEEE rounds it, the update alone
+                // does not
+                const float r = BITS == 8 ? sqrtf(v[j]) : sqrt_fast(v[j]);
+                p[j] = p[j] * decay -
+                       size * __fdividef(m[j], r * root + h.eps);
+                if (BITS == 8) v[j] = r;
             }
-        }
+            if (h.clamped) {
 #pragma unroll
-        for (int j = 0; j < kLane; j++) {
-            const float gj = g[j] * scale;
-            m[j] = m[j] * h.b1 + gj * h.omb1;
-            v[j] = v[j] * h.b2 + (gj * gj) * h.omb2;
-            const float r = sqrtf(v[j]);
-            float q = p[j] * decay - size * (m[j] / (r * root + h.eps));
-            q = q < h.lo ? h.lo : q;  // NaN stays
-            p[j] = q > h.hi ? h.hi : q;
-            if (BITS == 8) v[j] = r;
-        }
-        store_lane(pp, wide, mask, lane, p);
-        if (BITS == 32) {
-            store_lane(static_cast<float*>(t.m[ti]) + at, wide, mask, lane, m);
-            store_lane(static_cast<float*>(t.v[ti]) + at, wide, mask, lane, v);
-        } else {
-            const uint32_t q = b - t.first[ti];
-            uint32_t bits[kLane];
+                for (int j = 0; j < kLane; j++) {  // NaN stays
+                    p[j] = p[j] < h.lo ? h.lo : p[j];
+                    p[j] = p[j] > h.hi ? h.hi : p[j];
+                }
+            }
+            store_lane(p0 + at, wide, mask, lane, p);
+            if constexpr (BITS == 32) {
+                store_lane(m0 + at, wide, mask, lane, m);
+                store_lane(v0 + at, wide, mask, lane, v);
+            } else {
+                bool fm, fv;
+                const float tm = top_of(m, &fm), tv = top_of(v, &fv);
+                uint32_t bits[kLane];
+                const uint32_t place = key + uint32_t(at);
 #pragma unroll
-            for (int j = 0; j < kLane; j++)
-                bits[j] = wang_hash(key + uint32_t(at) +
-                                    (wide ? lane * kLane + j : lane + 32 * j));
-            bool fm, fv;
-            const float tm = top_of(m, &fm), tv = top_of(v, &fv);
-            store_codes(static_cast<uint8_t*>(t.m[ti]) + at, wide, mask, lane,
-                        encode<false>(m, 448.f / tm, fm, bits));
-            store_codes(static_cast<uint8_t*>(t.v[ti]) + at, wide, mask, lane,
-                        encode<true>(v, 448.f / tv, fv, bits));
-            if (lane == 0) {
-                t.sm[ti][q] = tm / 448.f;
-                t.sv[ti][q] = tv / 448.f;
+                for (int j = 0; j < kLane; j++)
+                    bits[j] = wang_hash(place + (wide ? lane * kLane + j
+                                                      : lane + 32 * j));
+                store_codes(m0 + at, wide, mask, lane,
+                            encode<false>(m, 448.f / tm, fm, bits));
+                store_codes(v0 + at, wide, mask, lane,
+                            encode<true>(v, 448.f / tv, fv, bits));
+                if (lane == 0) {
+                    sm[q] = tm / 448.f;
+                    sv[q] = tv / 448.f;
+                }
             }
         }
     }
@@ -545,6 +577,7 @@ void adamw_op(const AdamWArgs& a, cudaStream_t s) {
     h.ln_b2 = float(std::log(a.beta2));
     h.lo = a.clamp_lo;
     h.hi = a.clamp_hi;
+    h.clamped = a.clamp_lo > -INFINITY || a.clamp_hi < INFINITY;
     h.max_norm = float(a.max_norm);
     h.lr = a.lr;
     h.wd = a.weight_decay;
