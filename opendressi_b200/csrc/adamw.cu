@@ -6,8 +6,7 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // with g first scaled by min(1, max_norm / (norm + 1e-6)) when clipping, and p
-// clamped last. Every operation is rounded by itself, as in the plans' Adam.
-// Bound by memory: 28 bytes a value with f32 parameters and 32-bit moments,
+// clamped last. Bound by memory: 28 bytes a value with f32 parameters and 32-bit moments,
 // 16 + 8/256 with 8-bit ones.
 //
 // The tensors' addresses travel as a kernel argument (no table to upload, so
@@ -197,74 +196,85 @@ __device__ __forceinline__ void decode(uint2 c, float* o) {
     }
 }
 
-// The scale of a block's 8-bit values and 1 over it, from the largest finite
-// |x| of the warp. The floor keeps 448 / top finite.
+// The largest finite |x| of the warp's block, 2^-100 at least (448 over it
+// stays finite), and whether all of x is finite.
 __device__ __forceinline__ float top_of(const float* x, bool* finite) {
-    uint32_t top = 0u;
+    uint32_t u[kLane];
 #pragma unroll
     for (int j = 0; j < kLane; j++)
-        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+        u[j] = __float_as_uint(x[j]) & 0x7fffffffu;
+    uint32_t top = 0u;
+#pragma unroll
+    for (int j = 0; j < kLane; j += 2) top = __vimax3_u32(top, u[j], u[j + 1]);
     top = __reduce_max_sync(0xffffffffu, top);
     *finite = top < 0x7f800000u;
     if (!*finite) {
         top = 0u;
 #pragma unroll
-        for (int j = 0; j < kLane; j++) {
-            const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-            top = max(top, b < 0x7f800000u ? b : 0u);
-        }
+        for (int j = 0; j < kLane; j++)
+            top = max(top, u[j] < 0x7f800000u ? u[j] : 0u);
         top = __reduce_max_sync(0xffffffffu, top);
     }
     return fmaxf(__uint_as_float(top), 0x1p-100f);
 }
 
-// a in [0, 448 (1 + 2^-22)] up or down to a neighbouring e4m3 value (448 at
-// most: what two roundings left above it is cut), up with the probability of
-// its place between the two: 16 random bits (and a half) are added below the
-// 3 bits of fraction that stay. Below 2^-6 the values are 2^-9 apart, as they
-// are in [2^-6, 2^-5): the sum with 2^-6 is rounded instead.
-__device__ __forceinline__ float round_e4m3(float a, uint32_t bits16) {
-    const float lift = a < 0x1p-6f ? 0x1p-6f : 0.f;
-    const uint32_t b = __float_as_uint(a + lift) + (bits16 << 4 | 8u);
-    return __uint_as_float(b & 0xfff00000u) - lift;
+// The highest bytes of four words, the first's lowest.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t* b) {
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0073),
+                       __byte_perm(b[2], b[3], 0x0073), 0x5410);
 }
 
-// The codes of a lane's values x; ROOT: of values that are not negative and
-// do not become 0 unless they are.
+// The codes of a lane's values x, inv = 448 / the block's largest. ROOT: of
+// values that are not negative and do not become 0 unless they are.
+//
+// 2^-120 |x| inv, as the bits of a float, is an e4m3 number with 20 more bits
+// of fraction: the exponents of both then count from the same power of two,
+// and below 2^-6 (there 2^-126) both are equally spaced. 16 random bits and a
+// half are added to those 20 and what carries goes up: up with the probability
+// of the value's place between its neighbours. (All of it is moved up by 4
+// bits: a code is then a whole byte.) inv is within 3 * 2^-24 of its value:
+// the largest comes out below 448 + 8 * 2^-15 and never carries past 448.
 template <bool ROOT>
 __device__ __forceinline__ uint2 encode(const float* x, float inv, bool finite,
                                         const uint32_t* bits) {
-    uint32_t w[2] = {0u, 0u};
-    float a[kLane];
+    uint32_t b[kLane];
 #pragma unroll
     for (int j = 0; j < kLane; j++) {
-        a[j] = round_e4m3(fabsf(x[j]) * inv, ROOT ? bits[j] >> 16
-                                                  : bits[j] & 0xffffu);
-        if (ROOT) {
-            a[j] = x[j] > 0.f ? fmaxf(a[j], 0x1p-9f) : a[j];
-        } else {
-            a[j] = copysignf(a[j], x[j]);
-        }
+        // (two products as written: with -fmad=true nvcc 12.9 made zeros of
+        // fabsf(x[j]) * inv * 0x1p-120f here)
+        uint32_t z = __float_as_uint(
+                __fmul_rn(__fmul_rn(fabsf(x[j]), inv), 0x1p-120f));
+        // the smallest code where x > 0; what is no root of 0 has more bits
+        if (ROOT) z = max(z, min(__float_as_uint(x[j]), 1u << 20));
+        const uint32_t r = __byte_perm(bits[j], 0x80u, ROOT ? 0x7324 : 0x7104);
+        b[j] = z * 16u + r;
     }
     if (!finite) {
 #pragma unroll
         for (int j = 0; j < kLane; j++)
             if ((__float_as_uint(x[j]) & 0x7f800000u) == 0x7f800000u)
-                a[j] = __uint_as_float(0x7fc00000u);
+                b[j] = 0x7f000000u;  // NaN
     }
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        w[j / 2] |= uint32_t(__nv_cvt_float2_to_fp8x2(
-                            make_float2(a[2 * j], a[2 * j + 1]),
-                            __NV_SATFINITE, __NV_E4M3))
-                    << (j % 2 * 16);
-    return make_uint2(w[0], w[1]);
+    uint2 c = make_uint2(top_bytes(b), top_bytes(b + 4));
+    if (!ROOT) {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(x);
+        c.x |= top_bytes(u) & 0x80808080u;
+        c.y |= top_bytes(u + 4) & 0x80808080u;
+    }
+    return c;
 }
 
 // sqrt to 2^-23.
 __device__ __forceinline__ float sqrt_fast(float v) {
     float r;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// 1 / v to 2^-23, for v in [2^-126, 2^126] and 0.
+__device__ __forceinline__ float rcp_fast(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
 
@@ -366,13 +376,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
             for (int j = 0; j < kLane; j++) {
                 const float gj = g[j] * scale;
-                m[j] = m[j] * h.b1 + gj * h.omb1;
-                v[j] = v[j] * h.b2 + (gj * gj) * h.omb2;
-                // the codes want the root as IEEE rounds it, the update alone
-                // does not
-                const float r = BITS == 8 ? sqrtf(v[j]) : sqrt_fast(v[j]);
-                p[j] = p[j] * decay -
-                       size * __fdividef(m[j], r * root + h.eps);
+                m[j] = fmaf(m[j], h.b1, gj * h.omb1);
+                v[j] = fmaf(v[j], h.b2, (gj * gj) * h.omb2);
+                const float r = sqrt_fast(v[j]);
+                const float u = m[j] * rcp_fast(fmaf(r, root, h.eps));
+                p[j] = fmaf(-size, u, p[j] * decay);
                 if (BITS == 8) v[j] = r;
             }
             if (h.clamped) {
@@ -390,18 +398,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 bool fm, fv;
                 const float tm = top_of(m, &fm), tv = top_of(v, &fv);
                 uint32_t bits[kLane];
-                const uint32_t place = key + uint32_t(at);
+                const uint32_t place =
+                        key + uint32_t(at) + (wide ? lane * kLane : lane);
+                const uint32_t next = wide ? 1u : 32u;
 #pragma unroll
                 for (int j = 0; j < kLane; j++)
-                    bits[j] = wang_hash(place + (wide ? lane * kLane + j
-                                                      : lane + 32 * j));
+                    bits[j] = wang_hash(place + j * next);
                 store_codes(m0 + at, wide, mask, lane,
-                            encode<false>(m, 448.f / tm, fm, bits));
+                            encode<false>(m, 448.f * rcp_fast(tm), fm, bits));
                 store_codes(v0 + at, wide, mask, lane,
-                            encode<true>(v, 448.f / tv, fv, bits));
+                            encode<true>(v, 448.f * rcp_fast(tv), fv, bits));
                 if (lane == 0) {
-                    sm[q] = tm / 448.f;
-                    sv[q] = tv / 448.f;
+                    sm[q] = tm * (1.f / 448.f);
+                    sv[q] = tv * (1.f / 448.f);
                 }
             }
         }
