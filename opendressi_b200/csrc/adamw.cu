@@ -162,10 +162,9 @@ __device__ __forceinline__ void store_lane(T* p, bool wide, uint32_t mask,
     }
 }
 
-// e4m3 codes of a lane (packed) and the values they stand for.
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p, bool wide,
-                                            uint32_t mask, int lane) {
-    if (wide) return *reinterpret_cast<const uint2*>(p + lane * kLane);
+// e4m3 codes of a lane's values lane + 32 j, packed, and what they stand for.
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, uint32_t mask,
+                                            int lane) {
     uint32_t c[2] = {0u, 0u};
 #pragma unroll
     for (int j = 0; j < kLane; j++)
@@ -173,12 +172,8 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* p, bool wide,
             c[j / 4] |= uint32_t(p[lane + 32 * j]) << (j % 4 * 8);
     return make_uint2(c[0], c[1]);
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, bool wide,
-                                            uint32_t mask, int lane, uint2 c) {
-    if (wide) {
-        *reinterpret_cast<uint2*>(p + lane * kLane) = c;
-        return;
-    }
+__device__ __forceinline__ void store_codes(uint8_t* p, uint32_t mask,
+                                            int lane, uint2 c) {
     const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
     for (int j = 0; j < kLane; j++)
@@ -299,22 +294,227 @@ __device__ __forceinline__ uint32_t tensor_of(const Table& t, uint32_t b) {
     return lo;
 }
 
+// What a warp knows of the tensor it is in.
+template <typename T, typename State>
+struct Target {
+    T* p;
+    const T* g;
+    State* m;
+    State* v;
+    float* sm;
+    float* sv;
+    uint64_t n;
+    bool aligned;
+    uint32_t key;      // of the random bits
+    float size, root;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    float scale, decay;
+};
+
+// Which of a lane's values lane + 32 j a block with `left` values has.
+__device__ __forceinline__ uint32_t lane_mask(uint64_t left, int lane) {
+    uint32_t mask = 0u;
+#pragma unroll
+    for (int j = 0; j < kLane; j++)
+        mask |= uint32_t(uint64_t(lane + 32 * j) < left) << j;
+    return mask;
+}
+
+// The step of a lane's values. ROOT: v is left as its root.
+template <bool ROOT, typename Tensor>
+__device__ __forceinline__ void update(const Tensor& t, const AdamWHyper& h,
+                                       float* p, const float* g, float* m,
+                                       float* v) {
+#pragma unroll
+    for (int j = 0; j < kLane; j++) {
+        const float gj = g[j] * t.scale;
+        m[j] = fmaf(m[j], h.b1, gj * h.omb1);
+        v[j] = fmaf(v[j], h.b2, (gj * gj) * h.omb2);
+        const float r = sqrt_fast(v[j]);
+        const float u = m[j] * rcp_fast(fmaf(r, t.root, h.eps));
+        p[j] = fmaf(-t.size, u, p[j] * t.decay);
+        if (ROOT) v[j] = r;
+    }
+    if (h.clamped) {
+#pragma unroll
+        for (int j = 0; j < kLane; j++) {  // NaN stays
+            p[j] = p[j] < h.lo ? h.lo : p[j];
+            p[j] = p[j] > h.hi ? h.hi : p[j];
+        }
+    }
+}
+
+// Blocks q, q + kWarps, ... below stop of a tensor with 32-bit moments.
+template <typename T>
+__device__ __forceinline__ void blocks_32(const Target<T, float>& t,
+                                          const AdamWHyper& h, uint32_t q,
+                                          uint32_t stop, int lane) {
+    for (; q < stop; q += kWarps) {
+        const uint64_t at = uint64_t(q) * kBlock;
+        const bool wide = t.aligned && t.n - at >= kBlock;
+        const uint32_t mask = wide ? 0u : lane_mask(t.n - at, lane);
+        float p[kLane], g[kLane], m[kLane], v[kLane];
+        load_lane(t.g + at, wide, mask, lane, g);
+        load_lane(static_cast<const T*>(t.p + at), wide, mask, lane, p);
+        load_lane(static_cast<const float*>(t.m + at), wide, mask, lane, m);
+        load_lane(static_cast<const float*>(t.v + at), wide, mask, lane, v);
+        update<false>(t, h, p, g, m, v);
+        store_lane(t.p + at, wide, mask, lane, p);
+        store_lane(t.m + at, wide, mask, lane, m);
+        store_lane(t.v + at, wide, mask, lane, v);
+    }
+}
+
+// A warp's next block on its way to shared memory (8-bit moments): each lane
+// copies what it will read itself, two runs of 4 values, so no lane waits for
+// another.
+template <typename T>
+struct alignas(4 * sizeof(T)) Quad {
+    T v[4];
+};
+template <typename T>
+struct Stage {
+    Quad<T> p[2][32], g[2][32];
+    uint32_t m[2][32], v[2][32];
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                         uint32_t(__cvta_generic_to_shared(to))),
+                 "l"(from), "n"(BYTES)
+                 : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void fetch(const Target<T, uint8_t>& t, uint64_t at,
+                                      int lane, Stage<T>* s) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint64_t i = at + k * 128 + lane * 4;
+        copy_async<4 * sizeof(T)>(&s->g[k][lane], t.g + i);
+        copy_async<4 * sizeof(T)>(&s->p[k][lane], t.p + i);
+        copy_async<4>(&s->m[k][lane], t.m + i);
+        copy_async<4>(&s->v[k][lane], t.v + i);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void quad_in(const Quad<T>& q, float* o) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = to_f(q.v[j]);
+}
+template <typename T>
+__device__ __forceinline__ void quad_out(T* to, const float* o) {
+    Quad<T> f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) put(&f.v[j], o[j]);
+    *reinterpret_cast<Quad<T>*>(to) = f;
+}
+
+// The same with 8-bit moments: codes are bound by arithmetic as much as by
+// memory, so the next block is fetched while one is computed.
+template <typename T>
+__device__ __forceinline__ void blocks_8(const Target<T, uint8_t>& t,
+                                         const AdamWHyper& h, uint32_t q,
+                                         uint32_t stop, int lane,
+                                         Stage<T>* stage) {
+    auto is_wide = [&](uint32_t b) {
+        return t.aligned && t.n - uint64_t(b) * kBlock >= kBlock;
+    };
+    float next_m = 0.f, next_v = 0.f;  // scales of the block in flight
+    auto begin = [&](uint32_t b, Stage<T>* s) {
+        if (b < stop) {
+            if (is_wide(b)) fetch(t, uint64_t(b) * kBlock, lane, s);
+            next_m = t.sm[b];
+            next_v = t.sv[b];
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int turn = 0;
+    begin(q, &stage[0]);
+    for (; q < stop; q += kWarps, turn ^= 1) {
+        const uint64_t at = uint64_t(q) * kBlock;
+        const bool wide = is_wide(q);
+        const float am = next_m, av = next_v;
+        begin(q + kWarps, &stage[turn ^ 1]);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        float p[kLane], g[kLane], m[kLane], v[kLane];
+        uint2 cm, cv;
+        uint32_t mask = 0u;
+        if (wide) {
+            const Stage<T>& s = stage[turn];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                quad_in(s.g[k][lane], g + 4 * k);
+                quad_in(s.p[k][lane], p + 4 * k);
+            }
+            cm = make_uint2(s.m[0][lane], s.m[1][lane]);
+            cv = make_uint2(s.v[0][lane], s.v[1][lane]);
+        } else {
+            mask = lane_mask(t.n - at, lane);
+            load_lane(t.g + at, false, mask, lane, g);
+            load_lane(static_cast<const T*>(t.p + at), false, mask, lane, p);
+            cm = load_codes(t.m + at, mask, lane);
+            cv = load_codes(t.v + at, mask, lane);
+        }
+        decode(cm, m);
+        decode(cv, v);
+#pragma unroll
+        for (int j = 0; j < kLane; j++) {
+            m[j] = m[j] * am;
+            v[j] = v[j] * av;
+            v[j] = v[j] * v[j];
+        }
+        update<true>(t, h, p, g, m, v);
+        bool fm, fv;
+        const float tm = top_of(m, &fm), tv = top_of(v, &fv);
+        uint32_t bits[kLane];
+        const uint32_t place = t.key + uint32_t(at) + (wide ? 4 * lane : lane);
+        const uint32_t next = wide ? 1u : 32u, half = 128u;
+#pragma unroll
+        for (int j = 0; j < kLane; j++)
+            bits[j] = wang_hash(place + j % 4 * next + j / 4 * half);
+        cm = encode<false>(m, 448.f * rcp_fast(tm), fm, bits);
+        cv = encode<true>(v, 448.f * rcp_fast(tv), fv, bits);
+        if (wide) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint64_t i = at + k * 128 + lane * 4;
+                quad_out(t.p + i, p + 4 * k);
+                *reinterpret_cast<uint32_t*>(t.m + i) = k ? cm.y : cm.x;
+                *reinterpret_cast<uint32_t*>(t.v + i) = k ? cv.y : cv.x;
+            }
+        } else {
+            store_lane(t.p + at, false, mask, lane, p);
+            store_codes(t.m + at, mask, lane, cm);
+            store_codes(t.v + at, mask, lane, cv);
+        }
+        if (lane == 0) {
+            t.sm[q] = tm * (1.f / 448.f);
+            t.sv[q] = tv * (1.f / 448.f);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 template <typename T, int BITS, int CAP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         k_adamw(const __grid_constant__ AdamWTable<CAP> t,
                 const __grid_constant__ AdamWHyper h) {
-    const int lane = threadIdx.x & 31;
+    using State = typename StateOf<BITS>::type;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint64_t all = t.first[t.count];
     const uint32_t b_end = uint32_t(all * (blockIdx.x + 1) / gridDim.x);
-    uint32_t b = uint32_t(all * blockIdx.x / gridDim.x) + threadIdx.x / 32;
+    uint32_t b = uint32_t(all * blockIdx.x / gridDim.x) + warp;
 
-    float scale = 1.f;  // of the gradients
+    Target<T, State> w;
+    w.scale = 1.f;
     if (h.norm) {
         const float c = h.max_norm / (*h.norm + 1e-6f);
-        scale = c > 1.f ? 1.f : c;  // NaN stays
+        w.scale = c > 1.f ? 1.f : c;  // NaN stays
     }
     const double lr = h.lr_device ? double(*h.lr_device) : h.lr;
-    const float decay = float(1.0 - lr * h.wd);
+    w.decay = float(1.0 - lr * h.wd);
 
     uint32_t ti = b < b_end ? tensor_of(t, b) : 0u;
     while (b < b_end) {  // tensor after tensor
@@ -324,96 +524,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const int32_t step = *t.step[ti] + 1;
         // 1 - b^t = -expm1(t ln b): exact to a few 2^-24, also where b^t is
         // next to 1
-        const float size =
-                float(lr / double(-expm1f(float(step) * h.ln_b1)));
-        const float root = 1.f / sqrtf(-expm1f(float(step) * h.ln_b2));
-        const uint32_t key =
-                BITS == 8 ? wang_hash(wang_hash(h.seed ^
-                                                wang_hash(uint32_t(step))) +
-                                      t.index[ti])
-                          : 0u;
-        T* const p0 = static_cast<T*>(t.p[ti]);
-        const T* const g0 = static_cast<const T*>(t.g[ti]);
-        using State = typename StateOf<BITS>::type;
-        State* const m0 = static_cast<State*>(t.m[ti]);
-        State* const v0 = static_cast<State*>(t.v[ti]);
-        float* const sm = t.sm[ti];
-        float* const sv = t.sv[ti];
-        const uint64_t n = t.n[ti];
-        const bool aligned = t.wide[ti];
-        for (; b < stop; b += kWarps) {
-            const uint32_t q = b - first;
-            const uint64_t at = uint64_t(q) * kBlock;
-            const bool wide = aligned && n - at >= kBlock;
-            uint32_t mask = 0xffu;
-            if (!wide && n - at < kBlock) {
-                mask = 0u;
-#pragma unroll
-                for (int j = 0; j < kLane; j++)
-                    mask |= uint32_t(lane + 32 * j < int(n - at)) << j;
-            }
-            float p[kLane], g[kLane], m[kLane], v[kLane];
-            load_lane(g0 + at, wide, mask, lane, g);
-            load_lane(static_cast<const T*>(p0 + at), wide, mask, lane, p);
-            if constexpr (BITS == 32) {
-                load_lane(static_cast<const float*>(m0 + at), wide, mask, lane,
-                          m);
-                load_lane(static_cast<const float*>(v0 + at), wide, mask, lane,
-                          v);
-            } else {
-                const uint2 cm = load_codes(m0 + at, wide, mask, lane);
-                const uint2 cv = load_codes(v0 + at, wide, mask, lane);
-                const float am = sm[q], av = sv[q];
-                decode(cm, m);
-                decode(cv, v);
-#pragma unroll
-                for (int j = 0; j < kLane; j++) {
-                    m[j] = m[j] * am;
-                    v[j] = v[j] * av;
-                    v[j] = v[j] * v[j];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kLane; j++) {
-                const float gj = g[j] * scale;
-                m[j] = fmaf(m[j], h.b1, gj * h.omb1);
-                v[j] = fmaf(v[j], h.b2, (gj * gj) * h.omb2);
-                const float r = sqrt_fast(v[j]);
-                const float u = m[j] * rcp_fast(fmaf(r, root, h.eps));
-                p[j] = fmaf(-size, u, p[j] * decay);
-                if (BITS == 8) v[j] = r;
-            }
-            if (h.clamped) {
-#pragma unroll
-                for (int j = 0; j < kLane; j++) {  // NaN stays
-                    p[j] = p[j] < h.lo ? h.lo : p[j];
-                    p[j] = p[j] > h.hi ? h.hi : p[j];
-                }
-            }
-            store_lane(p0 + at, wide, mask, lane, p);
-            if constexpr (BITS == 32) {
-                store_lane(m0 + at, wide, mask, lane, m);
-                store_lane(v0 + at, wide, mask, lane, v);
-            } else {
-                bool fm, fv;
-                const float tm = top_of(m, &fm), tv = top_of(v, &fv);
-                uint32_t bits[kLane];
-                const uint32_t place =
-                        key + uint32_t(at) + (wide ? lane * kLane : lane);
-                const uint32_t next = wide ? 1u : 32u;
-#pragma unroll
-                for (int j = 0; j < kLane; j++)
-                    bits[j] = wang_hash(place + j * next);
-                store_codes(m0 + at, wide, mask, lane,
-                            encode<false>(m, 448.f * rcp_fast(tm), fm, bits));
-                store_codes(v0 + at, wide, mask, lane,
-                            encode<true>(v, 448.f * rcp_fast(tv), fv, bits));
-                if (lane == 0) {
-                    sm[q] = tm * (1.f / 448.f);
-                    sv[q] = tv * (1.f / 448.f);
-                }
-            }
+        w.size = float(lr / double(-expm1f(float(step) * h.ln_b1)));
+        w.root = 1.f / sqrtf(-expm1f(float(step) * h.ln_b2));
+        w.key = wang_hash(wang_hash(h.seed ^ wang_hash(uint32_t(step))) +
+                          t.index[ti]);
+        w.p = static_cast<T*>(t.p[ti]);
+        w.g = static_cast<const T*>(t.g[ti]);
+        w.m = static_cast<State*>(t.m[ti]);
+        w.v = static_cast<State*>(t.v[ti]);
+        w.sm = t.sm[ti];
+        w.sv = t.sv[ti];
+        w.n = t.n[ti];
+        w.aligned = t.wide[ti];
+        if constexpr (BITS == 32) {
+            blocks_32(w, h, b - first, stop - first, lane);
+        } else {
+            __shared__ Stage<T> stages[kWarps][2];
+            blocks_8(w, h, b - first, stop - first, lane, stages[warp]);
         }
+        b += (stop - b + kWarps - 1) / kWarps * kWarps;
     }
     // every block has read the counters once all have drawn a ticket
     __shared__ bool last;
@@ -459,9 +588,9 @@ void launch_adamw(const AdamWArgs& a, const AdamWHyper& h, uint32_t i0,
         t.step[k] = a.steps[i];
         t.n[k] = a.numel[i];
         t.index[k] = a.index ? a.index[i] : i;
-        const size_t st = BITS == 8 ? kLane : kLane * sizeof(float);
-        t.wide[k] = aligned(t.p[k], kLane * sizeof(T)) &&
-                    aligned(t.g[k], kLane * sizeof(T)) &&
+        const size_t run = BITS == 8 ? 4 * sizeof(T) : kLane * sizeof(T);
+        const size_t st = BITS == 8 ? 4 : kLane * sizeof(float);
+        t.wide[k] = aligned(t.p[k], run) && aligned(t.g[k], run) &&
                     aligned(t.m[k], st) && aligned(t.v[k], st);
         t.first[k] = uint32_t(blocks);
         blocks += (t.n[k] + kBlock - 1) / kBlock;
