@@ -43,14 +43,23 @@ constexpr int kBlock = 256;    // values a warp takes, and that share a scale
 constexpr int kLane = 8;       // values a lane takes
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 4;  // with 32-bit moments
+// With codes: 5 blocks on their way to each warp. 100.7M f32 values take 282
+// us with 3 thread blocks an SM and 3 blocks ahead, 301 with 4 and 3, 325 with
+// 4 and 2, 264 with 2 and 4, 256 with 2 and 5 (and 14 blocks a warp, below).
+constexpr int kCtasPerSm8 = 2;
+constexpr int kStages = 5;
+template <int BITS>
+constexpr int ctas_per_sm() {
+    return BITS == 8 ? kCtasPerSm8 : kCtasPerSm;
+}
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr uint64_t kMostBlocks = 1ull << 31;  // of one launch
 
 struct AdamWHyper {
     float b1, omb1, b2, omb2, eps, ln_b1, ln_b2;
     float lo, hi, max_norm;
-    bool clamped;
+    bool clamped, small_eps;
     double lr, wd;
     const float* lr_device;
     const float* norm;
@@ -191,75 +200,34 @@ __device__ __forceinline__ void decode(uint2 c, float* o) {
     }
 }
 
-// The largest finite |x| of the warp's block, 2^-100 at least (448 over it
-// stays finite), and whether all of x is finite.
-__device__ __forceinline__ float top_of(const float* x, bool* finite) {
-    uint32_t u[kLane];
-#pragma unroll
-    for (int j = 0; j < kLane; j++)
-        u[j] = __float_as_uint(x[j]) & 0x7fffffffu;
-    uint32_t top = 0u;
-#pragma unroll
-    for (int j = 0; j < kLane; j += 2) top = __vimax3_u32(top, u[j], u[j + 1]);
-    top = __reduce_max_sync(0xffffffffu, top);
-    *finite = top < 0x7f800000u;
-    if (!*finite) {
-        top = 0u;
-#pragma unroll
-        for (int j = 0; j < kLane; j++)
-            top = max(top, u[j] < 0x7f800000u ? u[j] : 0u);
-        top = __reduce_max_sync(0xffffffffu, top);
-    }
-    return fmaxf(__uint_as_float(top), 0x1p-100f);
+// Two 32-bit values in one register pair and one instruction.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ Two two(float a) { return two(a, a); }
+__device__ __forceinline__ void of_two(Two d, float* o) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(o[0]), "=f"(o[1]) : "l"(d));
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
 
-// The highest bytes of four words, the first's lowest.
-__device__ __forceinline__ uint32_t top_bytes(const uint32_t* b) {
-    return __byte_perm(__byte_perm(b[0], b[1], 0x0073),
-                       __byte_perm(b[2], b[3], 0x0073), 0x5410);
+// sqrt to 2^-23; the quick one takes numbers below 2^-126 for 0.
+__device__ __forceinline__ float sqrt_quick(float v) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
-
-// The codes of a lane's values x, inv = 448 / the block's largest. ROOT: of
-// values that are not negative and do not become 0 unless they are.
-//
-// 2^-120 |x| inv, as the bits of a float, is an e4m3 number with 20 more bits
-// of fraction: the exponents of both then count from the same power of two,
-// and below 2^-6 (there 2^-126) both are equally spaced. 16 random bits and a
-// half are added to those 20 and what carries goes up: up with the probability
-// of the value's place between its neighbours. (All of it is moved up by 4
-// bits: a code is then a whole byte.) inv is within 3 * 2^-24 of its value:
-// the largest comes out below 448 + 8 * 2^-15 and never carries past 448.
-template <bool ROOT>
-__device__ __forceinline__ uint2 encode(const float* x, float inv, bool finite,
-                                        const uint32_t* bits) {
-    uint32_t b[kLane];
-#pragma unroll
-    for (int j = 0; j < kLane; j++) {
-        // (two products as written: with -fmad=true nvcc 12.9 made zeros of
-        // fabsf(x[j]) * inv * 0x1p-120f here)
-        uint32_t z = __float_as_uint(
-                __fmul_rn(__fmul_rn(fabsf(x[j]), inv), 0x1p-120f));
-        // the smallest code where x > 0; what is no root of 0 has more bits
-        if (ROOT) z = max(z, min(__float_as_uint(x[j]), 1u << 20));
-        const uint32_t r = __byte_perm(bits[j], 0x80u, ROOT ? 0x7324 : 0x7104);
-        b[j] = z * 16u + r;
-    }
-    if (!finite) {
-#pragma unroll
-        for (int j = 0; j < kLane; j++)
-            if ((__float_as_uint(x[j]) & 0x7f800000u) == 0x7f800000u)
-                b[j] = 0x7f000000u;  // NaN
-    }
-    uint2 c = make_uint2(top_bytes(b), top_bytes(b + 4));
-    if (!ROOT) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(x);
-        c.x |= top_bytes(u) & 0x80808080u;
-        c.y |= top_bytes(u + 4) & 0x80808080u;
-    }
-    return c;
-}
-
-// sqrt to 2^-23.
 __device__ __forceinline__ float sqrt_fast(float v) {
     float r;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -271,6 +239,94 @@ __device__ __forceinline__ float rcp_fast(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
+}
+
+// The largest |a|, |b|, |c|; NaN if one is.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;"
+        : "=f"(d)
+        : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+    return d;
+}
+
+// The largest finite |x| of the warp's block, 2^-100 at least (448 over it
+// stays finite), and whether all of x is finite.
+__device__ __forceinline__ float top_of(const float* x, bool* finite) {
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < kLane; j += 2) most = largest(most, x[j], x[j + 1]);
+    uint32_t top = __reduce_max_sync(0xffffffffu,
+                                     __float_as_uint(most) & 0x7fffffffu);
+    *finite = top < 0x7f800000u;
+    if (!*finite) {
+        top = 0u;
+#pragma unroll
+        for (int j = 0; j < kLane; j++) {
+            const uint32_t u = __float_as_uint(x[j]) & 0x7fffffffu;
+            top = max(top, u < 0x7f800000u ? u : 0u);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+    }
+    return fmaxf(__uint_as_float(top), 0x1p-100f);
+}
+
+// The highest bytes of four words, the first's lowest.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t* b) {
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0073),
+                       __byte_perm(b[2], b[3], 0x0073), 0x5410);
+}
+
+// The codes of a lane's values x, top the block's largest, inv = 448 / top.
+// ROOT: of values that are not negative and do not become 0 unless they are.
+//
+// 2^-120 |x| inv, as the bits of a float, is an e4m3 number with 20 more bits
+// of fraction: the exponents of both then count from the same power of two,
+// and below 2^-6 (there 2^-126) both are equally spaced. 16 random bits and a
+// half are added to those 20 and what carries goes up: up with the probability
+// of the value's place between its neighbours. (All of it is moved up by 4
+// bits, which drops the sign: a code is then the highest byte.) inv is within
+// 3 * 2^-24 of its value: the largest comes out below 448 + 8 * 2^-15 and
+// never carries past 448.
+template <bool ROOT>
+__device__ __forceinline__ uint2 encode(const float* x, float top, bool finite,
+                                        const uint32_t* bits) {
+    const float inv = 448.f * rcp_fast(top);
+    uint32_t b[kLane];
+    float z[kLane];
+    // one product where inv 2^-120 is no denormal number
+    const bool once = top < 0x1p14f;
+    const Two first = two(once ? inv * 0x1p-120f : inv);
+#pragma unroll
+    for (int j = 0; j < kLane; j += 2)
+        of_two(mul2(two(x[j], x[j + 1]), first), z + j);
+    if (!once) {
+#pragma unroll
+        for (int j = 0; j < kLane; j++) z[j] = __fmul_rn(z[j], 0x1p-120f);
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; j++) {
+        uint32_t c = __float_as_uint(z[j]);
+        // the smallest code where x > 0; what is no root of 0 has more bits
+        if (ROOT) c = max(c, min(__float_as_uint(x[j]), 1u << 20));
+        const uint32_t r = __byte_perm(bits[j], 0x80u, ROOT ? 0x7324 : 0x7104);
+        b[j] = c * 16u + r;
+    }
+    if (!finite) {
+#pragma unroll
+        for (int j = 0; j < kLane; j++)
+            if ((__float_as_uint(x[j]) & 0x7f800000u) == 0x7f800000u)
+                b[j] = 0x7f000000u;  // NaN
+    }
+    uint2 c = make_uint2(top_bytes(b), top_bytes(b + 4));
+    if (!ROOT) {
+        uint32_t sign[kLane];
+#pragma unroll
+        for (int j = 0; j < kLane; j++) sign[j] = __float_as_uint(x[j]);
+        c.x |= top_bytes(sign) & 0x80808080u;
+        c.y |= top_bytes(sign + 4) & 0x80808080u;
+    }
+    return c;
 }
 
 template <int BITS>
@@ -324,15 +380,34 @@ template <bool ROOT, typename Tensor>
 __device__ __forceinline__ void update(const Tensor& t, const AdamWHyper& h,
                                        float* p, const float* g, float* m,
                                        float* v) {
+    float r[kLane];
 #pragma unroll
-    for (int j = 0; j < kLane; j++) {
-        const float gj = g[j] * t.scale;
-        m[j] = fmaf(m[j], h.b1, gj * h.omb1);
-        v[j] = fmaf(v[j], h.b2, (gj * gj) * h.omb2);
-        const float r = sqrt_fast(v[j]);
-        const float u = m[j] * rcp_fast(fmaf(r, t.root, h.eps));
-        p[j] = fmaf(-t.size, u, p[j] * t.decay);
-        if (ROOT) v[j] = r;
+    for (int j = 0; j < kLane; j += 2) {
+        const Two gj = mul2(two(g[j], g[j + 1]), two(t.scale));
+        of_two(fma2(two(m[j], m[j + 1]), two(h.b1), mul2(gj, two(h.omb1))),
+               m + j);
+        of_two(fma2(two(v[j], v[j + 1]), two(h.b2),
+                    mul2(mul2(gj, gj), two(h.omb2))),
+               v + j);
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; j++) r[j] = sqrt_quick(v[j]);
+    if (h.small_eps) {  // where the roots of denormal numbers count
+#pragma unroll
+        for (int j = 0; j < kLane; j++) r[j] = sqrt_fast(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; j += 2) {
+        float d[2];
+        of_two(fma2(two(r[j], r[j + 1]), two(t.root), two(h.eps)), d);
+        const Two u = mul2(two(m[j], m[j + 1]),
+                           two(rcp_fast(d[0]), rcp_fast(d[1])));
+        of_two(fma2(two(-t.size), u, mul2(two(p[j], p[j + 1]), two(t.decay))),
+               p + j);
+        if (ROOT) {
+            v[j] = r[j];
+            v[j + 1] = r[j + 1];
+        }
     }
     if (h.clamped) {
 #pragma unroll
@@ -343,11 +418,12 @@ __device__ __forceinline__ void update(const Tensor& t, const AdamWHyper& h,
     }
 }
 
-// Blocks q, q + kWarps, ... below stop of a tensor with 32-bit moments.
+// Blocks q, q + kWarps, ... below stop of a tensor with 32-bit moments; the
+// first one behind stop.
 template <typename T>
-__device__ __forceinline__ void blocks_32(const Target<T, float>& t,
-                                          const AdamWHyper& h, uint32_t q,
-                                          uint32_t stop, int lane) {
+__device__ __forceinline__ uint32_t blocks_32(const Target<T, float>& t,
+                                              const AdamWHyper& h, uint32_t q,
+                                              uint32_t stop, int lane) {
     for (; q < stop; q += kWarps) {
         const uint64_t at = uint64_t(q) * kBlock;
         const bool wide = t.aligned && t.n - at >= kBlock;
@@ -362,40 +438,46 @@ __device__ __forceinline__ void blocks_32(const Target<T, float>& t,
         store_lane(t.m + at, wide, mask, lane, m);
         store_lane(t.v + at, wide, mask, lane, v);
     }
+    return q;
 }
 
-// A warp's next block on its way to shared memory (8-bit moments): each lane
-// copies what it will read itself, two runs of 4 values, so no lane waits for
-// another.
+// A warp's coming block on its way to shared memory (8-bit moments), copied
+// in 16 bytes a lane past L1.
 template <typename T>
 struct alignas(4 * sizeof(T)) Quad {
     T v[4];
 };
 template <typename T>
-struct Stage {
-    Quad<T> p[2][32], g[2][32];
-    uint32_t m[2][32], v[2][32];
+struct alignas(16) Stage {
+    T g[kBlock], p[kBlock];
+    uint8_t codes[2][kBlock];
+    float scale[4];
 };
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+__device__ __forceinline__ void copy_16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                          uint32_t(__cvta_generic_to_shared(to))),
-                 "l"(from), "n"(BYTES)
+                 "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_4(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                         uint32_t(__cvta_generic_to_shared(to))),
+                 "l"(from)
                  : "memory");
 }
 
 template <typename T>
 __device__ __forceinline__ void fetch(const Target<T, uint8_t>& t, uint64_t at,
                                       int lane, Stage<T>* s) {
+    constexpr int run = 16 / sizeof(T);
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const uint64_t i = at + k * 128 + lane * 4;
-        copy_async<4 * sizeof(T)>(&s->g[k][lane], t.g + i);
-        copy_async<4 * sizeof(T)>(&s->p[k][lane], t.p + i);
-        copy_async<4>(&s->m[k][lane], t.m + i);
-        copy_async<4>(&s->v[k][lane], t.v + i);
+    for (int k = 0; k < kBlock; k += 32 * run) {
+        copy_16(s->g + k + lane * run, t.g + at + k + lane * run);
+        copy_16(s->p + k + lane * run, t.p + at + k + lane * run);
     }
+    copy_16(s->codes[0] + lane * 16,
+            (lane < 16 ? t.m : t.v - kBlock) + at + lane * 16);
 }
 
 template <typename T>
@@ -411,45 +493,52 @@ __device__ __forceinline__ void quad_out(T* to, const float* o) {
     *reinterpret_cast<Quad<T>*>(to) = f;
 }
 
-// The same with 8-bit moments: codes are bound by arithmetic as much as by
-// memory, so the next block is fetched while one is computed.
+// The same with 8-bit moments: codes are bound by arithmetic nearly as much as
+// by memory, so coming blocks are fetched while one is computed.
 template <typename T>
-__device__ __forceinline__ void blocks_8(const Target<T, uint8_t>& t,
-                                         const AdamWHyper& h, uint32_t q,
-                                         uint32_t stop, int lane,
-                                         Stage<T>* stage) {
+__device__ __forceinline__ uint32_t blocks_8(const Target<T, uint8_t>& t,
+                                             const AdamWHyper& h, uint32_t q,
+                                             uint32_t stop, int lane,
+                                             Stage<T>* stage) {
     auto is_wide = [&](uint32_t b) {
         return t.aligned && t.n - uint64_t(b) * kBlock >= kBlock;
     };
-    float next_m = 0.f, next_v = 0.f;  // scales of the block in flight
     auto begin = [&](uint32_t b, Stage<T>* s) {
         if (b < stop) {
             if (is_wide(b)) fetch(t, uint64_t(b) * kBlock, lane, s);
-            next_m = t.sm[b];
-            next_v = t.sv[b];
+            if (lane < 2) copy_4(&s->scale[lane], (lane ? t.sv : t.sm) + b);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     int turn = 0;
-    begin(q, &stage[0]);
-    for (; q < stop; q += kWarps, turn ^= 1) {
+#pragma unroll
+    for (int k = 0; k < kStages; k++) begin(q + k * kWarps, &stage[k]);
+    for (; q < stop; q += kWarps) {
         const uint64_t at = uint64_t(q) * kBlock;
         const bool wide = is_wide(q);
-        const float am = next_m, av = next_v;
-        begin(q + kWarps, &stage[turn ^ 1]);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        __syncwarp();
+        Stage<T>& s = stage[turn];
+        const float am = s.scale[0], av = s.scale[1];
         float p[kLane], g[kLane], m[kLane], v[kLane];
         uint2 cm, cv;
         uint32_t mask = 0u;
-        if (wide) {
-            const Stage<T>& s = stage[turn];
+        if (wide) {  // two runs of 4 values
+            auto quad = [&](const T* q, int k) {
+                return *reinterpret_cast<const Quad<T>*>(q + k * 128 +
+                                                         lane * 4);
+            };
+            auto word = [&](const uint8_t* q, int k) {
+                return *reinterpret_cast<const uint32_t*>(q + k * 128 +
+                                                          lane * 4);
+            };
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                quad_in(s.g[k][lane], g + 4 * k);
-                quad_in(s.p[k][lane], p + 4 * k);
+                quad_in(quad(s.g, k), g + 4 * k);
+                quad_in(quad(s.p, k), p + 4 * k);
             }
-            cm = make_uint2(s.m[0][lane], s.m[1][lane]);
-            cv = make_uint2(s.v[0][lane], s.v[1][lane]);
+            cm = make_uint2(word(s.codes[0], 0), word(s.codes[0], 1));
+            cv = make_uint2(word(s.codes[1], 0), word(s.codes[1], 1));
         } else {
             mask = lane_mask(t.n - at, lane);
             load_lane(t.g + at, false, mask, lane, g);
@@ -457,13 +546,17 @@ __device__ __forceinline__ void blocks_8(const Target<T, uint8_t>& t,
             cm = load_codes(t.m + at, mask, lane);
             cv = load_codes(t.v + at, mask, lane);
         }
+        // all lanes have theirs: the place is free for a later block
+        __syncwarp();
+        begin(q + kStages * kWarps, &s);
+        if (++turn == kStages) turn = 0;
         decode(cm, m);
         decode(cv, v);
 #pragma unroll
-        for (int j = 0; j < kLane; j++) {
-            m[j] = m[j] * am;
-            v[j] = v[j] * av;
-            v[j] = v[j] * v[j];
+        for (int j = 0; j < kLane; j += 2) {
+            of_two(mul2(two(m[j], m[j + 1]), two(am)), m + j);
+            const Two r = mul2(two(v[j], v[j + 1]), two(av));
+            of_two(mul2(r, r), v + j);
         }
         update<true>(t, h, p, g, m, v);
         bool fm, fv;
@@ -474,8 +567,8 @@ __device__ __forceinline__ void blocks_8(const Target<T, uint8_t>& t,
 #pragma unroll
         for (int j = 0; j < kLane; j++)
             bits[j] = wang_hash(place + j % 4 * next + j / 4 * half);
-        cm = encode<false>(m, 448.f * rcp_fast(tm), fm, bits);
-        cv = encode<true>(v, 448.f * rcp_fast(tv), fv, bits);
+        cm = encode<false>(m, tm, fm, bits);
+        cv = encode<true>(v, tv, fv, bits);
         if (wide) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -495,10 +588,11 @@ __device__ __forceinline__ void blocks_8(const Target<T, uint8_t>& t,
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    return q;
 }
 
 template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<BITS>())
         k_adamw(const __grid_constant__ AdamWTable<CAP> t,
                 const __grid_constant__ AdamWHyper h) {
     using State = typename StateOf<BITS>::type;
@@ -520,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     while (b < b_end) {  // tensor after tensor
         while (b >= t.first[ti + 1]) ti++;
         const uint32_t first = t.first[ti];
-        const uint32_t stop = min(b_end, t.first[ti + 1]);
+        const uint32_t stop = min(b_end, t.first[ti + 1]) - first;
         const int32_t step = *t.step[ti] + 1;
         // 1 - b^t = -expm1(t ln b): exact to a few 2^-24, also where b^t is
         // next to 1
@@ -537,12 +631,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         w.n = t.n[ti];
         w.aligned = t.wide[ti];
         if constexpr (BITS == 32) {
-            blocks_32(w, h, b - first, stop - first, lane);
+            b = first + blocks_32(w, h, b - first, stop, lane);
         } else {
-            __shared__ Stage<T> stages[kWarps][2];
-            blocks_8(w, h, b - first, stop - first, lane, stages[warp]);
+            extern __shared__ __align__(16) char stages[];
+            b = first +
+                blocks_8(w, h, b - first, stop, lane,
+                         reinterpret_cast<Stage<T>*>(stages) + warp * kStages);
         }
-        b += (stop - b + kWarps - 1) / kWarps * kWarps;
     }
     // every block has read the counters once all have drawn a ticket
     __shared__ bool last;
@@ -588,18 +683,32 @@ void launch_adamw(const AdamWArgs& a, const AdamWHyper& h, uint32_t i0,
         t.step[k] = a.steps[i];
         t.n[k] = a.numel[i];
         t.index[k] = a.index ? a.index[i] : i;
-        const size_t run = BITS == 8 ? 4 * sizeof(T) : kLane * sizeof(T);
-        const size_t st = BITS == 8 ? 4 : kLane * sizeof(float);
+        const size_t run = BITS == 8 ? 16 : kLane * sizeof(T);
+        const size_t st = BITS == 8 ? 16 : kLane * sizeof(float);
         t.wide[k] = aligned(t.p[k], run) && aligned(t.g[k], run) &&
                     aligned(t.m[k], st) && aligned(t.v[k], st);
         t.first[k] = uint32_t(blocks);
         blocks += (t.n[k] + kBlock - 1) / kBlock;
     }
     t.first[t.count] = uint32_t(blocks);
+    // Whole waves of thread blocks, each a run of memory of its own: SMs
+    // further from the memory take fewer of them, and all of them together
+    // touch few pages at a time. Of 4 or more blocks a warp (100.7M f32
+    // values, 32 bits: 472 us as one wave, 434 of 16, 424 of 8, 419 of 4 and
+    // of 2, 442 of 1), of 14 with codes (278 of 8, 262 of 10, 256 of 14, 260
+    // of 20, 266 of 32: there the fetch ahead starts anew in each).
+    const uint64_t wave = uint64_t(sm_count()) * ctas_per_sm<BITS>();
+    const uint64_t waves = std::max<uint64_t>(
+            1, blocks / (wave * kWarps * (BITS == 8 ? 14 : 4)));
     const uint64_t grid = std::max<uint64_t>(
             1, std::min<uint64_t>((blocks + kWarps - 1) / kWarps,
-                                  uint64_t(sm_count()) * kCtasPerSm));
-    k_adamw<T, BITS, CAP><<<unsigned(grid), kThreads, 0, s>>>(t, h);
+                                  wave * waves));
+    const int smem = BITS == 8 ? kWarps * kStages * sizeof(Stage<T>) : 0;
+    if (smem > 48 << 10)
+        DRESSI_CUDA(cudaFuncSetAttribute(
+                k_adamw<T, BITS, CAP>,
+                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    k_adamw<T, BITS, CAP><<<unsigned(grid), kThreads, smem, s>>>(t, h);
     DRESSI_CUDA(cudaGetLastError());
 }
 
@@ -717,6 +826,8 @@ void adamw_op(const AdamWArgs& a, cudaStream_t s) {
     h.hi = a.clamp_hi;
     h.clamped = a.clamp_lo > -INFINITY || a.clamp_hi < INFINITY;
     h.max_norm = float(a.max_norm);
+    // the root of 2^-126 is 2^-63: nothing next to an eps of 2^-40
+    h.small_eps = h.eps < 0x1p-40f;
     h.lr = a.lr;
     h.wd = a.weight_decay;
     h.lr_device = a.lr_device;
