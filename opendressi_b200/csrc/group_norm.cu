@@ -34,7 +34,7 @@ namespace dressi {
 
 namespace {
 
-constexpr int kGnThreads = 512;
+constexpr int kGnThreads = 256;
 
 struct GnDims {
     uint64_t n, rows;
@@ -46,7 +46,8 @@ struct GnDims {
     int pieces;        // slabs per group (1 unless a group exceeds a slab)
     uint32_t chunks;   // row chunks of a sample
     uint64_t chunk_rows;
-    int threads;       // threads that work (flat: a multiple of a row cover)
+    int threads;       // flat: threads that work (they cover whole rows)
+    int lanes;         // flat: rows they cover
 };
 
 template <typename T>
@@ -96,26 +97,27 @@ __device__ __forceinline__ void slab_of(const GnDims& d, int s, int* col0,
 // What a thread walks over: values base, base + step, ... below end of a
 // sample, each VEC wide; its first value is column `col` of the slab.
 struct Walk {
-    uint64_t base, step, end;
+    uint64_t base, step;
     int col0, cols, lanes, col;
+    uint32_t steps;
     bool works;
 };
 
+// Blocks are (slab, chunk) along x and samples along y.
 template <int VEC>
-__device__ __forceinline__ Walk walk_of(const GnDims& d, int slab,
-                                        uint32_t chunk) {
+__device__ __forceinline__ Walk walk_of(const GnDims& d, uint32_t chunk,
+                                        int slab) {
     Walk w;
     const uint64_t r0 = uint64_t(chunk) * d.chunk_rows;
-    const uint64_t r1 = min(r0 + d.chunk_rows, d.rows);
-    w.end = r1 * d.C;
+    const uint64_t end = min(r0 + d.chunk_rows, d.rows) * d.C;
     if (d.slabs == 1) {
         w.col0 = 0;
         w.cols = d.C;
-        w.lanes = int(int64_t(d.threads) * VEC / d.C);
+        w.lanes = d.lanes;
         w.works = int(threadIdx.x) < d.threads;
-        w.base = r0 * d.C + uint64_t(threadIdx.x) * VEC;
+        w.base = r0 * d.C + threadIdx.x * VEC;
         w.step = uint64_t(d.threads) * VEC;
-        w.col = int(uint32_t(threadIdx.x) * VEC % uint32_t(d.C));
+        w.col = int(threadIdx.x * VEC % uint32_t(d.C));
     } else {
         slab_of(d, slab, &w.col0, &w.cols);
         const int per_row = w.cols / VEC;
@@ -126,40 +128,125 @@ __device__ __forceinline__ Walk walk_of(const GnDims& d, int slab,
         w.base = (r0 + lane) * d.C + w.col0 + w.col;
         w.step = uint64_t(w.lanes) * d.C;
     }
+    w.steps = 0;
+    if (w.works && w.base < end) {
+        const uint64_t left = end - w.base + w.step - 1;
+        w.steps = left >> 32 ? uint32_t(left / w.step)
+                             : uint32_t(left) / uint32_t(w.step);
+    }
     return w;
 }
 
-// Number of steps of the walk that starts at base.
-__device__ __forceinline__ uint32_t steps_of(const Walk& w, uint64_t base) {
-    return base < w.end ? uint32_t((w.end - base + w.step - 1) / w.step) : 0u;
+// Calls fn(j, channel, group) for the values of a thread's vector.
+template <int VEC, typename F>
+__device__ __forceinline__ void each_channel(const GnDims& d, const Walk& w,
+                                             F&& fn) {
+    int c = w.col0 + w.col, g = c / d.cpg, k = c - g * d.cpg;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+        fn(j, c, g);
+        if (++c == w.col0 + w.cols) {  // rows of a flat walk follow each other
+            c = w.col0;
+            g = c / d.cpg;
+            k = c - g * d.cpg;
+        } else if (++k == d.cpg) {
+            k = 0;
+            g++;
+        }
+    }
 }
 
 // Rounding below 0 is 0; NaN stays.
 __device__ __forceinline__ float nonneg(float v) { return v < 0.f ? 0.f : v; }
 
-struct Moments {
-    double n, mean, m2;
-};
-__device__ __forceinline__ void merge(Moments* a, double n, double mean,
-                                      double m2) {
-    if (n == 0.0) return;
-    const double t = a->n + n, d = mean - a->mean;
-    a->mean += d * (n / t);
-    a->m2 += m2 + d * d * (a->n * (n / t));
-    a->n = t;
-}
-__device__ __forceinline__ void merge_warp(Moments* a) {
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const double n = __shfl_xor_sync(0xffffffffu, a->n, o);
-        const double mean = __shfl_xor_sync(0xffffffffu, a->mean, o);
-        const double m2 = __shfl_xor_sync(0xffffffffu, a->m2, o);
-        // both sides in one order: the same bits in every lane
-        const bool up = threadIdx.x & o;
-        Moments lo = up ? Moments{n, mean, m2} : *a;
-        const Moments hi = up ? *a : Moments{n, mean, m2};
-        merge(&lo, hi.n, hi.mean, hi.m2);
-        *a = lo;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Vectors that are on their way to a thread at a time, of each image.
+constexpr int kGnAhead = 8;
+
+template <typename T, int VEC>
+constexpr bool whole_vectors() {
+    return VEC * sizeof(T) == 16;
+}
+// Bytes of shared memory of a block that walks over `images`.
+template <typename T, int VEC>
+constexpr int ring_bytes(int images) {
+    return whole_vectors<T, VEC>() ? images * kGnAhead * kGnThreads * 16 : 0;
+}
+
+__device__ __forceinline__ void copy_16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         uint32_t(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
+}
+
+// Calls fn(t, a, b) for the vectors t = 0 .. steps - 1 of one image (q null)
+// or two. Whole vectors come through a ring in shared memory, each thread's
+// its own: loads in registers would be a quarter as many.
+template <typename T, int VEC, int IMAGES, typename F>
+__device__ __forceinline__ void walk_over(const T* p, const T* q,
+                                          uint64_t step, uint32_t steps,
+                                          char* ring, F&& fn) {
+    using V = Pack<T, VEC>;
+    if constexpr (whole_vectors<T, VEC>()) {
+        V* own = reinterpret_cast<V*>(ring) + threadIdx.x;
+        V* const own_end = own + kGnAhead * IMAGES * kGnThreads;
+        uint32_t sent = 0;
+        auto send = [&](V* to) {
+            if (sent < steps) {
+                copy_16(to, p);
+                p += step;
+                if (IMAGES == 2) {
+                    copy_16(to + kGnThreads, q);
+                    q += step;
+                }
+            }
+            sent++;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int k = 0; k < kGnAhead; k++)
+            send(own + k * IMAGES * kGnThreads);
+        V* slot = own;
+        for (uint32_t t = 0; t < steps; t++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kGnAhead - 1)
+                         : "memory");
+            const V a = *slot, b = IMAGES == 2 ? slot[kGnThreads] : V{};
+            send(slot);
+            slot += IMAGES * kGnThreads;
+            if (slot == own_end) slot = own;
+            fn(t, a, b);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+        constexpr int kBatch = 4 / IMAGES;  // loads under way together
+        uint32_t t = 0;
+        for (; t + kBatch <= steps; t += kBatch) {
+            V a[kBatch], b[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; k++) {
+                a[k] = load_pack<T, VEC>(p + k * step);
+                if (IMAGES == 2) b[k] = load_pack<T, VEC>(q + k * step);
+            }
+            p += kBatch * step;
+            if (IMAGES == 2) q += kBatch * step;
+#pragma unroll
+            for (int k = 0; k < kBatch; k++) fn(t + k, a[k], b[k]);
+        }
+        for (; t < steps; t++, p += step) {
+            const V a = load_pack<T, VEC>(p);
+            V b{};
+            if (IMAGES == 2) {
+                b = load_pack<T, VEC>(q);
+                q += step;
+            }
+            fn(t, a, b);
+        }
     }
 }
 
@@ -186,137 +273,168 @@ __device__ __forceinline__ float act_grad(float dy, float z) {
 // ------------------------------------------------------------------ forward
 
 // Statistics of one (sample, chunk, slab): part[n][g][chunk * pieces + piece]
-// = (mean less the group's first value in the sample, sum of squares about
-// the mean). Means of 1e4 deviations would lose digits of the variance in 32
-// bits; their distances from a common value do not.
+// = (mean, sum of squares about it). A thread sums distances from its own
+// first value; the group's mean is an average of the threads' means, its sum
+// of squares theirs plus count times (their mean - the mean)^2 (the pairwise
+// update of Chan, Golub and LeVeque, all at once). Means enter as distances
+// from one of them: of 1e4 deviations they keep no digits of the variance in
+// 32 bits.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kGnThreads)
-        k_gn_stats(GnDims d, const T* x, float2* part) {
+        k_gn_stats(GnDims d, const T* __restrict__ x,
+                   double2* __restrict__ part) {
+    extern __shared__ __align__(16) char ring[];
     __shared__ float2 sm[kGnThreads * VEC];
     __shared__ uint32_t cnt[kGnThreads];
-    uint64_t i = blockIdx.x;
-    const int slab = int(i % d.slabs);
-    i /= d.slabs;
-    const uint32_t chunk = uint32_t(i % d.chunks);
-    const uint64_t n = i / d.chunks;
-    const Walk w = walk_of<VEC>(d, slab, chunk);
-    const T* xs = x + n * d.rows * d.C;
-    float k[VEC], s1[VEC], s2[VEC], k0[VEC];
-    const uint32_t steps = w.works ? steps_of(w, w.base) : 0u;
-    if (steps > 0) {
-        const Pack<T, VEC> f = load_pack<T, VEC>(xs + w.base);
-        int c = w.col;
+    const int slab = d.slabs == 1 ? 0 : int(blockIdx.x % uint32_t(d.slabs));
+    const uint32_t chunk =
+            d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
+    const uint64_t n = blockIdx.y;
+    const Walk w = walk_of<VEC>(d, chunk, slab);
+    if (w.steps > 0) {
+        float k[VEC], s1[VEC], s2[VEC];
+        walk_over<T, VEC, 1>(
+                x + n * d.rows * d.C + w.base, static_cast<const T*>(nullptr),
+                w.step, w.steps, ring,
+                [&](uint32_t t, const Pack<T, VEC>& v, const Pack<T, VEC>&) {
+                    if (t == 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            k[j] = to_f<T>(f.v[j]);
-            s1[j] = s2[j] = 0.f;
-            k0[j] = to_f<T>(xs[(w.col0 + c) / d.cpg * d.cpg]);
-            if (++c == w.cols) c = 0;
-        }
-        const T* p = xs + w.base;
-#pragma unroll 4
-        for (uint32_t t = 1; t < steps; t++) {
-            p += w.step;
-            const Pack<T, VEC> v = load_pack<T, VEC>(p);
+                        for (int j = 0; j < VEC; j++) {
+                            k[j] = to_f<T>(v.v[j]);
+                            s1[j] = s2[j] = 0.f;
+                        }
+                        return;
+                    }
 #pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                const float e = to_f<T>(v.v[j]) - k[j];
-                s1[j] += e;
-                s2[j] += e * e;
-            }
-        }
-        const float inv = 1.f / float(steps);
+                    for (int j = 0; j < VEC; j++) {
+                        const float e = to_f<T>(v.v[j]) - k[j];
+                        s1[j] += e;
+                        s2[j] += e * e;
+                    }
+                });
+        const float inv = 1.f / float(w.steps);
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
             const float m = s1[j] * inv;
             sm[threadIdx.x * VEC + j] =
-                    make_float2(k[j] - k0[j] + m, nonneg(s2[j] - s1[j] * m));
+                    make_float2(k[j] + m, nonneg(s2[j] - s1[j] * m));
         }
     }
-    cnt[threadIdx.x] = steps;
+    cnt[threadIdx.x] = w.steps;
     __syncthreads();
     // sm[lane * cols + c]: one warp per group merges its lanes x channels
     const int per = d.pieces > 1 ? w.cols : d.cpg;
-    const int groups = w.cols / per, g0 = w.col0 / d.cpg;
+    const int groups = d.pieces > 1 ? 1 : w.cols / per, g0 = w.col0 / d.cpg;
     for (int g = threadIdx.x / 32; g < groups; g += kGnThreads / 32) {
-        Moments a{0.0, 0.0, 0.0};
-        for (int e = threadIdx.x & 31; e < w.lanes * per; e += 32) {
-            const int at = e / per * w.cols + g * per + e % per;
-            const float2 v = sm[at];
-            merge(&a, double(cnt[at / VEC]), v.x, v.y);
-        }
-        merge_warp(&a);
+        const float ref = sm[g * per].x;
+        double count = 0.0, sum = 0.0, m2 = 0.0;
+        auto each = [&](auto&& fn) {
+            // e = lane * per + channel, 32 at a time
+            int l = int(threadIdx.x & 31) / per;
+            int c = int(threadIdx.x & 31) - l * per;
+            const int dl = 32 / per, dc = 32 - dl * per;
+            while (l < w.lanes) {
+                const int at = l * w.cols + g * per + c;
+                const uint32_t n = cnt[at / VEC];
+                if (n > 0) fn(float(n), sm[at]);
+                l += dl;
+                c += dc;
+                if (c >= per) {
+                    c -= per;
+                    l++;
+                }
+            }
+        };
+        each([&](float n, float2 v) {
+            count += n;
+            sum += double(n) * double(v.x - ref);
+        });
+        count = warp_sum(count);
+        const double off = warp_sum(sum) / count;
+        const float off32 = float(off);
+        each([&](float n, float2 v) {
+            const float e = v.x - ref - off32;
+            m2 += double(v.y) + double(n * e) * double(e);
+        });
+        m2 = warp_sum(m2);
         if ((threadIdx.x & 31) == 0)
             part[(n * d.G + g0 + g) * d.chunks * d.pieces +
                  size_t(chunk) * d.pieces + slab % d.pieces] =
-                    make_float2(float(a.mean), float(a.m2));
+                    make_double2(double(ref) + off, m2);
     }
 }
 
 // mean[n][g], rstd[n][g] from the parts; one warp each.
-template <typename T>
-__global__ void k_gn_finish(GnDims d, uint64_t n, const T* x,
-                            const float2* part, float* mean, float* rstd) {
+__global__ void k_gn_finish(GnDims d, uint32_t n,
+                            const double2* __restrict__ part,
+                            float* __restrict__ mean,
+                            float* __restrict__ rstd) {
     const uint64_t i = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-    if (i >= n * d.G) return;
-    Moments a{0.0, 0.0, 0.0};
+    if (i >= uint64_t(n) * d.G) return;
     const uint32_t np = d.chunks * d.pieces;
+    const double2* own = part + i * np;
+    auto count_of = [&](uint32_t e) {
+        uint32_t chunk = e, piece = 0;
+        if (d.pieces > 1) {
+            chunk = e / d.pieces;
+            piece = e - chunk * d.pieces;
+        }
+        const uint64_t rows = min(d.chunk_rows, d.rows - chunk * d.chunk_rows);
+        return double(rows) *
+               (d.pieces > 1
+                        ? min(d.slab_cols, d.cpg - int(piece) * d.slab_cols)
+                        : d.cpg);
+    };
+    const double all = double(d.rows) * d.cpg;
+    double sum = 0.0, m2 = 0.0;
+    for (uint32_t e = threadIdx.x & 31; e < np; e += 32)
+        sum += count_of(e) * own[e].x;
+    const double mu = warp_sum(sum) / all;
     for (uint32_t e = threadIdx.x & 31; e < np; e += 32) {
-        const uint32_t chunk = e / d.pieces, piece = e % d.pieces;
-        const uint64_t r0 = chunk * d.chunk_rows;
-        const uint64_t rows = min(d.chunk_rows, d.rows - r0);
-        const int cols = d.pieces > 1
-                                 ? min(d.slab_cols,
-                                       d.cpg - int(piece) * d.slab_cols)
-                                 : d.cpg;
-        const float2 v = part[i * np + e];
-        merge(&a, double(rows) * cols, v.x, v.y);
+        const double off = own[e].x - mu;
+        m2 += own[e].y + count_of(e) * off * off;
     }
-    merge_warp(&a);
+    m2 = warp_sum(m2);
     if ((threadIdx.x & 31) == 0) {
-        const T first = x[i / d.G * d.rows * d.C + i % d.G * d.cpg];
-        mean[i] = float(a.mean + to_f<T>(first));
-        rstd[i] = float(1.0 / sqrt(a.m2 / a.n + double(d.eps)));
+        mean[i] = float(mu);
+        rstd[i] = float(1.0 / sqrt(m2 / all + double(d.eps)));
     }
 }
 
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(kGnThreads)
-        k_gn_apply(GnDims d, const T* x, const float* weight,
-                   const float* bias, const float* mean, const float* rstd,
-                   T* y) {
+        k_gn_apply(GnDims d, const T* __restrict__ x,
+                   const float* __restrict__ weight,
+                   const float* __restrict__ bias,
+                   const float* __restrict__ mean,
+                   const float* __restrict__ rstd, T* __restrict__ y) {
+    extern __shared__ __align__(16) char ring[];
     // the last chunks first: they are what the statistics pass left on chip
-    uint64_t i = gridDim.x - 1 - blockIdx.x;
-    const int slab = int(i % d.slabs);
-    i /= d.slabs;
-    const uint32_t chunk = uint32_t(i % d.chunks);
-    const uint64_t n = i / d.chunks;
-    const Walk w = walk_of<VEC>(d, slab, chunk);
-    if (!w.works) return;
-    const T* xs = x + n * d.rows * d.C;
-    T* ys = y + n * d.rows * d.C;
+    const uint32_t i = gridDim.x - 1 - blockIdx.x;
+    const uint64_t n = gridDim.y - 1 - blockIdx.y;
+    const int slab = d.slabs == 1 ? 0 : int(i % uint32_t(d.slabs));
+    const uint32_t chunk = d.slabs == 1 ? i : i / uint32_t(d.slabs);
+    const Walk w = walk_of<VEC>(d, chunk, slab);
+    if (w.steps == 0) return;
     float mu[VEC], a[VEC], b[VEC];
-    int c = w.col;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) {
-        const int ch = w.col0 + c, g = ch / d.cpg;
+    each_channel<VEC>(d, w, [&](int j, int c, int g) {
         mu[j] = mean[n * d.G + g];
-        a[j] = rstd[n * d.G + g] * (weight ? weight[ch] : 1.f);
-        b[j] = bias ? bias[ch] : 0.f;
-        if (++c == w.cols) c = 0;
-    }
-    const uint32_t steps = steps_of(w, w.base);
-    uint64_t at = w.base;
-#pragma unroll 4
-    for (uint32_t t = 0; t < steps; t++, at += w.step) {
-        const Pack<T, VEC> v = load_pack<T, VEC>(xs + at);
-        Pack<T, VEC> o;
+        a[j] = rstd[n * d.G + g] * (weight ? weight[c] : 1.f);
+        b[j] = bias ? bias[c] : 0.f;
+    });
+    T* to = y + n * d.rows * d.C + w.base;
+    walk_over<T, VEC, 1>(
+            x + n * d.rows * d.C + w.base, static_cast<const T*>(nullptr),
+            w.step, w.steps, ring,
+            [&](uint32_t, const Pack<T, VEC>& v, const Pack<T, VEC>&) {
+                Pack<T, VEC> o;
 #pragma unroll
-        for (int j = 0; j < VEC; j++)
-            o.v[j] = from_f<T>(
-                    act_<ACT>((to_f<T>(v.v[j]) - mu[j]) * a[j] + b[j]));
-        *reinterpret_cast<Pack<T, VEC>*>(ys + at) = o;
-    }
+                for (int j = 0; j < VEC; j++)
+                    o.v[j] = from_f<T>(act_<ACT>(
+                            (to_f<T>(v.v[j]) - mu[j]) * a[j] + b[j]));
+                *reinterpret_cast<Pack<T, VEC>*>(to) = o;
+                to += w.step;
+            });
 }
 
 // ----------------------------------------------------------------- backward
@@ -324,46 +442,42 @@ __global__ void __launch_bounds__(kGnThreads)
 // part[n][chunk][c] = (sum dz, sum dz h) over the chunk's rows.
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(kGnThreads)
-        k_gn_grad_sums(GnDims d, const T* dy, const T* x, const float* weight,
-                       const float* bias, const float* mean,
-                       const float* rstd, float2* part) {
+        k_gn_grad_sums(GnDims d, const T* __restrict__ dy,
+                       const T* __restrict__ x,
+                       const float* __restrict__ weight,
+                       const float* __restrict__ bias,
+                       const float* __restrict__ mean,
+                       const float* __restrict__ rstd,
+                       float2* __restrict__ part) {
+    extern __shared__ __align__(16) char ring[];
     __shared__ float2 sm[kGnThreads * VEC];
-    uint64_t i = blockIdx.x;
-    const int slab = int(i % d.slabs);
-    i /= d.slabs;
-    const uint32_t chunk = uint32_t(i % d.chunks);
-    const uint64_t n = i / d.chunks;
-    const Walk w = walk_of<VEC>(d, slab, chunk);
-    const T* xs = x + n * d.rows * d.C;
-    const T* gs = dy + n * d.rows * d.C;
+    const int slab = d.slabs == 1 ? 0 : int(blockIdx.x % uint32_t(d.slabs));
+    const uint32_t chunk =
+            d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
+    const uint64_t n = blockIdx.y;
+    const Walk w = walk_of<VEC>(d, chunk, slab);
     if (w.works) {
         float mu[VEC], r[VEC], wt[VEC], b[VEC], A[VEC], B[VEC];
-        int c = w.col;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            const int ch = w.col0 + c, g = ch / d.cpg;
+        each_channel<VEC>(d, w, [&](int j, int c, int g) {
             mu[j] = mean[n * d.G + g];
             r[j] = rstd[n * d.G + g];
-            wt[j] = weight ? weight[ch] : 1.f;
-            b[j] = bias ? bias[ch] : 0.f;
+            wt[j] = weight ? weight[c] : 1.f;
+            b[j] = bias ? bias[c] : 0.f;
             A[j] = B[j] = 0.f;
-            if (++c == w.cols) c = 0;
-        }
-        const uint32_t steps = steps_of(w, w.base);
-        uint64_t at = w.base;
-#pragma unroll 2
-        for (uint32_t t = 0; t < steps; t++, at += w.step) {
-            const Pack<T, VEC> v = load_pack<T, VEC>(xs + at);
-            const Pack<T, VEC> e = load_pack<T, VEC>(gs + at);
+        });
+        const uint64_t at = n * d.rows * d.C + w.base;
+        walk_over<T, VEC, 2>(
+                x + at, dy + at, w.step, w.steps, ring,
+                [&](uint32_t, const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
 #pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                const float h = (to_f<T>(v.v[j]) - mu[j]) * r[j];
-                const float dz =
-                        act_grad<ACT>(to_f<T>(e.v[j]), h * wt[j] + b[j]);
-                A[j] += dz;
-                B[j] += dz * h;
-            }
-        }
+                    for (int j = 0; j < VEC; j++) {
+                        const float h = (to_f<T>(v.v[j]) - mu[j]) * r[j];
+                        const float dz = act_grad<ACT>(to_f<T>(e.v[j]),
+                                                       h * wt[j] + b[j]);
+                        A[j] += dz;
+                        B[j] += dz * h;
+                    }
+                });
 #pragma unroll
         for (int j = 0; j < VEC; j++)
             sm[threadIdx.x * VEC + j] = make_float2(A[j], B[j]);
@@ -437,49 +551,47 @@ __global__ void __launch_bounds__(512)
 
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(kGnThreads)
-        k_gn_grad_apply(GnDims d, const T* dy, const T* x,
-                        const float* weight, const float* bias,
-                        const float* mean, const float* rstd,
-                        const float2* means, T* dx) {
-    uint64_t i = gridDim.x - 1 - blockIdx.x;
-    const int slab = int(i % d.slabs);
-    i /= d.slabs;
-    const uint32_t chunk = uint32_t(i % d.chunks);
-    const uint64_t n = i / d.chunks;
-    const Walk w = walk_of<VEC>(d, slab, chunk);
-    if (!w.works) return;
-    const T* xs = x + n * d.rows * d.C;
-    const T* gs = dy + n * d.rows * d.C;
-    T* os = dx + n * d.rows * d.C;
+        k_gn_grad_apply(GnDims d, const T* __restrict__ dy,
+                        const T* __restrict__ x,
+                        const float* __restrict__ weight,
+                        const float* __restrict__ bias,
+                        const float* __restrict__ mean,
+                        const float* __restrict__ rstd,
+                        const float2* __restrict__ means,
+                        T* __restrict__ dx) {
+    extern __shared__ __align__(16) char ring[];
+    const uint32_t i = gridDim.x - 1 - blockIdx.x;
+    const uint64_t n = gridDim.y - 1 - blockIdx.y;
+    const int slab = d.slabs == 1 ? 0 : int(i % uint32_t(d.slabs));
+    const uint32_t chunk = d.slabs == 1 ? i : i / uint32_t(d.slabs);
+    const Walk w = walk_of<VEC>(d, chunk, slab);
+    if (w.steps == 0) return;
     float mu[VEC], r[VEC], wt[VEC], b[VEC], ma[VEC], mb[VEC];
-    int c = w.col;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) {
-        const int ch = w.col0 + c, g = ch / d.cpg;
+    each_channel<VEC>(d, w, [&](int j, int c, int g) {
         mu[j] = mean[n * d.G + g];
         r[j] = rstd[n * d.G + g];
-        wt[j] = weight ? weight[ch] : 1.f;
-        b[j] = bias ? bias[ch] : 0.f;
+        wt[j] = weight ? weight[c] : 1.f;
+        b[j] = bias ? bias[c] : 0.f;
         const float2 m = means[n * d.G + g];
         ma[j] = m.x;
         mb[j] = m.y;
-        if (++c == w.cols) c = 0;
-    }
-    const uint32_t steps = steps_of(w, w.base);
-    uint64_t at = w.base;
-#pragma unroll 2
-    for (uint32_t t = 0; t < steps; t++, at += w.step) {
-        const Pack<T, VEC> v = load_pack<T, VEC>(xs + at);
-        const Pack<T, VEC> e = load_pack<T, VEC>(gs + at);
-        Pack<T, VEC> o;
+    });
+    const uint64_t at = n * d.rows * d.C + w.base;
+    T* to = dx + at;
+    walk_over<T, VEC, 2>(
+            x + at, dy + at, w.step, w.steps, ring,
+            [&](uint32_t, const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
+                Pack<T, VEC> o;
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            const float h = (to_f<T>(v.v[j]) - mu[j]) * r[j];
-            const float dz = act_grad<ACT>(to_f<T>(e.v[j]), h * wt[j] + b[j]);
-            o.v[j] = from_f<T>(r[j] * (wt[j] * dz - ma[j] - h * mb[j]));
-        }
-        *reinterpret_cast<Pack<T, VEC>*>(os + at) = o;
-    }
+                for (int j = 0; j < VEC; j++) {
+                    const float h = (to_f<T>(v.v[j]) - mu[j]) * r[j];
+                    const float dz =
+                            act_grad<ACT>(to_f<T>(e.v[j]), h * wt[j] + b[j]);
+                    o.v[j] = from_f<T>(r[j] * (wt[j] * dz - ma[j] - h * mb[j]));
+                }
+                *reinterpret_cast<Pack<T, VEC>*>(to) = o;
+                to += w.step;
+            });
 }
 
 // dweight[c], dbias[c] = the sums over samples (in order).
@@ -543,6 +655,7 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
         const uint64_t want = (sample / vec + cover - 1) / cover;
         d.threads = cover * int(std::min<uint64_t>(kGnThreads / cover,
                                                    std::max<uint64_t>(want, 1)));
+        d.lanes = int(int64_t(d.threads) * vec / a.C);
         row_unit = vec / std::gcd(a.C, vec);
     } else {
         // slabs start at multiples of the vector in a row of such
@@ -570,9 +683,9 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     p.vec = vec;
     const uint64_t bytes = std::max<uint64_t>(1, sample * es * (grad ? 2 : 1));
     p.batch = std::min<uint64_t>(std::max<uint64_t>(1, kGnRoundBytes / bytes),
-                                 a.n);
-    // two resident blocks an SM, one wave; a thread takes 4 steps or more
-    const uint64_t wave = 148 * 2;
+                                 std::min<uint64_t>(a.n, 65535));
+    // one wave of resident blocks; a thread takes 4 steps or more
+    const uint64_t wave = 148 * (grad ? 3 : 4);
     uint64_t chunks = std::max<uint64_t>(
             1, wave / std::max<uint64_t>(1, p.batch * d.slabs));
     const uint64_t lanes = std::max<uint64_t>(
@@ -583,15 +696,12 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     d.chunk_rows = (a.rows + chunks - 1) / chunks;
     d.chunk_rows = (d.chunk_rows + row_unit - 1) / row_unit * row_unit;
     d.chunks = uint32_t((a.rows + d.chunk_rows - 1) / d.chunk_rows);
-    // a launch's blocks fit the grid
-    const uint64_t per = uint64_t(d.chunks) * d.slabs;
-    p.batch = std::max<uint64_t>(
-            1, std::min<uint64_t>(p.batch, ((1ull << 31) - 1) / per));
     return p;
 }
 
 struct GnWorkspace {
-    float2* part;
+    double2* part;  // forward
+    float2* sums_part;
     float* mean;
     float* rstd;
     float2* sums;
@@ -608,16 +718,26 @@ GnWorkspace carve(const GroupNormArgs& a, const GnPlan& p, bool grad,
     GnWorkspace w{};
     const size_t nb = size_t(p.batch), parts = size_t(p.d.chunks);
     if (grad) {
-        w.part = ar.take<float2>(nb * parts * a.C);
+        w.sums_part = ar.take<float2>(nb * parts * a.C);
         w.sums = ar.take<float2>(size_t(a.n) * a.C);
         w.means = ar.take<float2>(size_t(a.n) * a.G);
     } else {
-        w.part = ar.take<float2>(nb * a.G * parts * p.d.pieces);
+        w.part = ar.take<double2>(nb * a.G * parts * p.d.pieces);
         w.mean = ar.take<float>(size_t(a.n) * a.G);
         w.rstd = ar.take<float>(size_t(a.n) * a.G);
     }
     w.bytes = ar.used;
     return w;
+}
+
+// Launches a kernel with a ring of `smem` bytes.
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 grid, int smem, cudaStream_t s,
+            A... args) {
+    DRESSI_CUDA(cudaFuncSetAttribute(
+            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<grid, kGnThreads, smem, s>>>(args...);
+    DRESSI_CUDA(cudaGetLastError());
 }
 
 template <typename T, int VEC>
@@ -627,28 +747,21 @@ void forward_t(const GnPlan& p, const GroupNormArgs& a, const void* x,
     const size_t sample = size_t(a.rows) * a.C;
     for (uint64_t n0 = 0; n0 < a.n; n0 += p.batch) {
         const uint64_t nb = std::min<uint64_t>(p.batch, a.n - n0);
-        const unsigned grid = unsigned(nb * p.d.chunks * p.d.slabs);
+        const dim3 grid(p.d.chunks * p.d.slabs, unsigned(nb));
         const T* xb = static_cast<const T*>(x) + n0 * sample;
         T* yb = static_cast<T*>(y) + n0 * sample;
         float* mb = mean + n0 * a.G;
         float* rb = rstd + n0 * a.G;
-        k_gn_stats<T, VEC><<<grid, kGnThreads, 0, s>>>(p.d, xb, w.part);
-        k_gn_finish<T><<<unsigned((nb * a.G + 7) / 8), 256, 0, s>>>(
-                p.d, nb, xb, w.part, mb, rb);
-        switch (a.act) {
-            case 1:
-                k_gn_apply<T, VEC, 1><<<grid, kGnThreads, 0, s>>>(
-                        p.d, xb, weight, bias, mb, rb, yb);
-                break;
-            case 2:
-                k_gn_apply<T, VEC, 2><<<grid, kGnThreads, 0, s>>>(
-                        p.d, xb, weight, bias, mb, rb, yb);
-                break;
-            default:
-                k_gn_apply<T, VEC, 0><<<grid, kGnThreads, 0, s>>>(
-                        p.d, xb, weight, bias, mb, rb, yb);
-        }
-        DRESSI_CUDA(cudaGetLastError());
+        constexpr int smem = ring_bytes<T, VEC>(1);
+        launch(k_gn_stats<T, VEC>, grid, smem, s, p.d, xb, w.part);
+        k_gn_finish<<<unsigned((nb * a.G + 7) / 8), 256, 0, s>>>(
+                p.d, uint32_t(nb), w.part, mb, rb);
+        launch(a.act == 1   ? k_gn_apply<T, VEC, 1>
+               : a.act == 2 ? k_gn_apply<T, VEC, 2>
+                            : k_gn_apply<T, VEC, 0>,
+               grid, smem, s, p.d, xb, weight, bias,
+               static_cast<const float*>(mb), static_cast<const float*>(rb),
+               yb);
     }
 }
 
@@ -663,21 +776,22 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
     const int bundles = (a.G + bundle - 1) / bundle;
     for (uint64_t n0 = 0; n0 < a.n; n0 += p.batch) {
         const uint64_t nb = std::min<uint64_t>(p.batch, a.n - n0);
-        const unsigned grid = unsigned(nb * p.d.chunks * p.d.slabs);
+        const dim3 grid(p.d.chunks * p.d.slabs, unsigned(nb));
         const T* xb = static_cast<const T*>(x) + n0 * sample;
         const T* gb = static_cast<const T*>(dy) + n0 * sample;
         const float* mb = mean + n0 * a.G;
         const float* rb = rstd + n0 * a.G;
         float2* means = w.means + n0 * a.G;
-        k_gn_grad_sums<T, VEC, ACT><<<grid, kGnThreads, 0, s>>>(
-                p.d, gb, xb, weight, bias, mb, rb, w.part);
+        constexpr int smem = ring_bytes<T, VEC>(2);
+        launch(k_gn_grad_sums<T, VEC, ACT>, grid, smem, s, p.d, gb, xb, weight,
+               bias, mb, rb, w.sums_part);
         k_gn_grad_finish<<<unsigned(nb * bundles), 512, 0, s>>>(
-                p.d, bundle, w.part, weight, w.sums + n0 * a.C, means);
-        if (dx)
-            k_gn_grad_apply<T, VEC, ACT><<<grid, kGnThreads, 0, s>>>(
-                    p.d, gb, xb, weight, bias, mb, rb, means,
-                    static_cast<T*>(dx) + n0 * sample);
+                p.d, bundle, w.sums_part, weight, w.sums + n0 * a.C, means);
         DRESSI_CUDA(cudaGetLastError());
+        if (dx)
+            launch(k_gn_grad_apply<T, VEC, ACT>, grid, smem, s, p.d, gb, xb,
+                   weight, bias, mb, rb, static_cast<const float2*>(means),
+                   static_cast<T*>(dx) + n0 * sample);
     }
     if (dweight || dbias) {
         k_gn_grad_affine<<<unsigned((a.C + 127) / 128), 128, 0, s>>>(
