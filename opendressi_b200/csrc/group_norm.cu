@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <numeric>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -48,6 +49,7 @@ struct GnDims {
     uint64_t chunk_rows;
     int threads;       // flat: threads that work (they cover whole rows)
     int lanes;         // flat: rows they cover
+    int run;           // channels of a group that a vector holds side by side
 };
 
 template <typename T>
@@ -79,6 +81,86 @@ struct alignas(sizeof(T) * VEC) Pack {
 template <typename T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
     return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+
+// Two 32-bit values in one register pair and one instruction.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ Two two(float a) { return two(a, a); }
+__device__ __forceinline__ float2 of_two(Two d) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(d));
+    return f;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// A vector as pairs of 32-bit values (one and a zero where VEC is 1).
+template <int VEC>
+constexpr int kPairs = (VEC + 1) / 2;
+
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& v, Two* o) {
+    if constexpr (VEC == 1) {
+        o[0] = two(to_f<T>(v.v[0]), 0.f);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; k++) {
+            if constexpr (sizeof(T) == 4) {
+                o[k] = two(v.v[2 * k], v.v[2 * k + 1]);
+            } else {
+                const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[k];
+                if constexpr (std::is_same<T, __half>::value) {
+                    const float2 f = __half22float2(
+                            *reinterpret_cast<const __half2*>(&w));
+                    o[k] = two(f.x, f.y);
+                } else {
+                    o[k] = two(__uint_as_float(w << 16),
+                               __uint_as_float(w & 0xffff0000u));
+                }
+            }
+        }
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> pack(const Two* o) {
+    Pack<T, VEC> v;
+    if constexpr (VEC == 1) {
+        v.v[0] = from_f<T>(of_two(o[0]).x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; k++) {
+            const float2 f = of_two(o[k]);
+            if constexpr (sizeof(T) == 4) {
+                v.v[2 * k] = f.x;
+                v.v[2 * k + 1] = f.y;
+            } else if constexpr (std::is_same<T, __half>::value) {
+                reinterpret_cast<__half2*>(&v)[k] =
+                        __floats2half2_rn(f.x, f.y);
+            } else {
+                reinterpret_cast<__nv_bfloat162*>(&v)[k] =
+                        __floats2bfloat162_rn(f.x, f.y);
+            }
+        }
+    }
+    return v;
 }
 
 // Columns [col0, col0 + cols) of slab s.
@@ -159,23 +241,27 @@ __device__ __forceinline__ void each_channel(const GnDims& d, const Walk& w,
 // Rounding below 0 is 0; NaN stays.
 __device__ __forceinline__ float nonneg(float v) { return v < 0.f ? 0.f : v; }
 
-__device__ __forceinline__ double warp_sum(double v) {
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// Vectors that are on their way to a thread at a time, of each image.
-constexpr int kGnAhead = 8;
+// Stages on their way to a thread at a time, of two vectors of each image.
+constexpr int kGnStages = 4;
 
 template <typename T, int VEC>
 constexpr bool whole_vectors() {
     return VEC * sizeof(T) == 16;
 }
 // Bytes of shared memory of a block that walks over `images`.
+// (and then writes VEC pairs of sums there).
 template <typename T, int VEC>
 constexpr int ring_bytes(int images) {
-    return whole_vectors<T, VEC>() ? images * kGnAhead * kGnThreads * 16 : 0;
+    return whole_vectors<T, VEC>()
+                   ? images * kGnStages * 2 * kGnThreads * 16
+                   : VEC * kGnThreads * int(sizeof(float2));
 }
 
 __device__ __forceinline__ void copy_16(void* to, const void* from) {
@@ -185,42 +271,53 @@ __device__ __forceinline__ void copy_16(void* to, const void* from) {
                  : "memory");
 }
 
-// Calls fn(t, a, b) for the vectors t = 0 .. steps - 1 of one image (q null)
-// or two. Whole vectors come through a ring in shared memory, each thread's
-// its own: loads in registers would be a quarter as many.
+// Calls fn(a, b) for `steps` vectors of one image (q null) or two. Whole
+// vectors come through a ring in shared memory, each thread's its own: loads
+// into registers would be a quarter as many.
 template <typename T, int VEC, int IMAGES, typename F>
 __device__ __forceinline__ void walk_over(const T* p, const T* q,
                                           uint64_t step, uint32_t steps,
                                           char* ring, F&& fn) {
     using V = Pack<T, VEC>;
     if constexpr (whole_vectors<T, VEC>()) {
+        constexpr int stage = 2 * IMAGES * kGnThreads;
         V* own = reinterpret_cast<V*>(ring) + threadIdx.x;
-        V* const own_end = own + kGnAhead * IMAGES * kGnThreads;
         uint32_t sent = 0;
         auto send = [&](V* to) {
-            if (sent < steps) {
+            if (sent + 1 < steps) {
                 copy_16(to, p);
-                p += step;
+                copy_16(to + kGnThreads, p + step);
+                p += 2 * step;
                 if (IMAGES == 2) {
-                    copy_16(to + kGnThreads, q);
-                    q += step;
+                    copy_16(to + 2 * kGnThreads, q);
+                    copy_16(to + 3 * kGnThreads, q + step);
+                    q += 2 * step;
                 }
+            } else if (sent < steps) {
+                copy_16(to, p);
+                if (IMAGES == 2) copy_16(to + 2 * kGnThreads, q);
             }
-            sent++;
+            sent += 2;
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int k = 0; k < kGnAhead; k++)
-            send(own + k * IMAGES * kGnThreads);
+        for (int k = 0; k < kGnStages; k++) send(own + k * stage);
         V* slot = own;
-        for (uint32_t t = 0; t < steps; t++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kGnAhead - 1)
+        for (uint32_t t = 0; t < steps; t += 2) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kGnStages - 1)
                          : "memory");
-            const V a = *slot, b = IMAGES == 2 ? slot[kGnThreads] : V{};
-            send(slot);
-            slot += IMAGES * kGnThreads;
-            if (slot == own_end) slot = own;
-            fn(t, a, b);
+            const V a = *slot, b = IMAGES == 2 ? slot[2 * kGnThreads] : V{};
+            if (t + 1 < steps) {
+                const V a1 = slot[kGnThreads];
+                const V b1 = IMAGES == 2 ? slot[3 * kGnThreads] : V{};
+                send(slot);
+                fn(a, b);
+                fn(a1, b1);
+            } else {
+                fn(a, b);
+            }
+            slot += stage;
+            if (slot == own + kGnStages * stage) slot = own;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
@@ -236,7 +333,7 @@ __device__ __forceinline__ void walk_over(const T* p, const T* q,
             p += kBatch * step;
             if (IMAGES == 2) q += kBatch * step;
 #pragma unroll
-            for (int k = 0; k < kBatch; k++) fn(t + k, a[k], b[k]);
+            for (int k = 0; k < kBatch; k++) fn(a[k], b[k]);
         }
         for (; t < steps; t++, p += step) {
             const V a = load_pack<T, VEC>(p);
@@ -245,27 +342,41 @@ __device__ __forceinline__ void walk_over(const T* p, const T* q,
                 b = load_pack<T, VEC>(q);
                 q += step;
             }
-            fn(t, a, b);
+            fn(a, b);
         }
     }
 }
 
 // act 0: none, 1: relu, 2: silu. NaN stays NaN.
-__device__ __forceinline__ float sigmoid_(float z) {
-    return __fdividef(1.f, 1.f + __expf(-z));
+__device__ __forceinline__ Two sigmoid2(Two z) {
+    const float2 t = of_two(mul2(z, two(-1.4426950408889634f)));
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = of_two(add2(two(e.x, e.y), two(1.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+    return two(e.x, e.y);
 }
 template <int ACT>
-__device__ __forceinline__ float act_(float z) {
-    if (ACT == 1) return z < 0.f ? 0.f : z;
-    if (ACT == 2) return z * sigmoid_(z);
+__device__ __forceinline__ Two act2(Two z) {
+    if (ACT == 1) {
+        const float2 f = of_two(z);
+        return two(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);
+    }
+    if (ACT == 2) return mul2(z, sigmoid2(z));
     return z;
 }
 template <int ACT>
-__device__ __forceinline__ float act_grad(float dy, float z) {
-    if (ACT == 1) return z <= 0.f ? 0.f : dy;
-    if (ACT == 2) {
-        const float s = sigmoid_(z);
-        return dy * (s * (1.f + z * (1.f - s)));
+__device__ __forceinline__ Two act_grad2(Two dy, Two z) {
+    if (ACT == 1) {
+        const float2 f = of_two(z), g = of_two(dy);
+        return two(f.x <= 0.f ? 0.f : g.x, f.y <= 0.f ? 0.f : g.y);
+    }
+    if (ACT == 2) {  // s (1 + z (1 - s))
+        const Two s = sigmoid2(z);
+        const Two t = fma2(s, two(-1.f), two(1.f));
+        return mul2(dy, mul2(s, fma2(z, t, two(1.f))));
     }
     return dy;
 }
@@ -274,69 +385,99 @@ __device__ __forceinline__ float act_grad(float dy, float z) {
 
 // Statistics of one (sample, chunk, slab): part[n][g][chunk * pieces + piece]
 // = (mean, sum of squares about it). A thread sums distances from its own
-// first value; the group's mean is an average of the threads' means, its sum
-// of squares theirs plus count times (their mean - the mean)^2 (the pairwise
-// update of Chan, Golub and LeVeque, all at once). Means enter as distances
-// from one of them: of 1e4 deviations they keep no digits of the variance in
-// 32 bits.
+// first value; runs of `run` channels of a group are merged in the thread, the
+// threads' results by a warp a group: the group's mean is an average of
+// theirs, its sum of squares theirs plus count times (their mean - the mean)^2
+// (the pairwise update of Chan, Golub and LeVeque, all at once). Means enter
+// as distances from one of them: of 1e4 deviations they keep no digits of the
+// variance in 32 bits.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kGnThreads)
         k_gn_stats(GnDims d, const T* __restrict__ x,
                    double2* __restrict__ part) {
     extern __shared__ __align__(16) char ring[];
-    __shared__ float2 sm[kGnThreads * VEC];
     __shared__ uint32_t cnt[kGnThreads];
     const int slab = d.slabs == 1 ? 0 : int(blockIdx.x % uint32_t(d.slabs));
     const uint32_t chunk =
             d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
     const uint64_t n = blockIdx.y;
     const Walk w = walk_of<VEC>(d, chunk, slab);
+    constexpr int P = kPairs<VEC>;
+    float mean[2 * P], m2[2 * P];
     if (w.steps > 0) {
-        float k[VEC], s1[VEC], s2[VEC];
+        Two k[P], s1[P], s2[P];
+        const T* own = x + n * d.rows * d.C + w.base;
+        unpack<T, VEC>(load_pack<T, VEC>(own), k);
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            k[j] = mul2(k[j], two(-1.f));
+            s1[j] = s2[j] = two(0.f);
+        }
         walk_over<T, VEC, 1>(
-                x + n * d.rows * d.C + w.base, static_cast<const T*>(nullptr),
-                w.step, w.steps, ring,
-                [&](uint32_t t, const Pack<T, VEC>& v, const Pack<T, VEC>&) {
-                    if (t == 0) {
+                own, static_cast<const T*>(nullptr), w.step, w.steps, ring,
+                [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) {
+                    Two e[P];
+                    unpack<T, VEC>(v, e);
 #pragma unroll
-                        for (int j = 0; j < VEC; j++) {
-                            k[j] = to_f<T>(v.v[j]);
-                            s1[j] = s2[j] = 0.f;
-                        }
-                        return;
-                    }
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const float e = to_f<T>(v.v[j]) - k[j];
-                        s1[j] += e;
-                        s2[j] += e * e;
+                    for (int j = 0; j < P; j++) {
+                        e[j] = add2(e[j], k[j]);
+                        s1[j] = add2(s1[j], e[j]);
+                        s2[j] = fma2(e[j], e[j], s2[j]);
                     }
                 });
         const float inv = 1.f / float(w.steps);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            const float m = s1[j] * inv;
-            sm[threadIdx.x * VEC + j] =
-                    make_float2(k[j] + m, nonneg(s2[j] - s1[j] * m));
+        for (int j = 0; j < P; j++) {
+            const Two m = mul2(s1[j], two(inv));
+            const float2 q = of_two(fma2(mul2(s1[j], two(-1.f)), m, s2[j]));
+            const float2 c = of_two(add2(m, mul2(k[j], two(-1.f))));
+            mean[2 * j] = c.x;
+            mean[2 * j + 1] = c.y;
+            m2[2 * j] = nonneg(q.x);
+            m2[2 * j + 1] = nonneg(q.y);
         }
+        // neighbours of a group: equal counts
+        float half = 0.5f * float(w.steps);
+#pragma unroll
+        for (int h = 1; h < VEC; h *= 2) {
+            if (h < d.run) {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 2 * h) {
+                    const float e = mean[j + h] - mean[j];
+                    m2[j] += m2[j + h] + e * e * half;
+                    mean[j] += 0.5f * e;
+                }
+                half *= 2.f;
+            }
+        }
+    }
+    // the ring is free once every thread has left it
+    __syncthreads();
+    float2* const sm = reinterpret_cast<float2*>(ring);
+    if (w.steps > 0) {
+        const int at = int(threadIdx.x) * (VEC / d.run);
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+            if ((j & (d.run - 1)) == 0)
+                sm[at + j / d.run] = make_float2(mean[j], m2[j]);
     }
     cnt[threadIdx.x] = w.steps;
     __syncthreads();
-    // sm[lane * cols + c]: one warp per group merges its lanes x channels
-    const int per = d.pieces > 1 ? w.cols : d.cpg;
-    const int groups = d.pieces > 1 ? 1 : w.cols / per, g0 = w.col0 / d.cpg;
+    // sm[lane * cols + c] with runs for columns
+    const int cols = w.cols / d.run, runs = VEC / d.run;
+    const int per = d.pieces > 1 ? cols : d.cpg / d.run;
+    const int groups = d.pieces > 1 ? 1 : cols / per, g0 = w.col0 / d.cpg;
     for (int g = threadIdx.x / 32; g < groups; g += kGnThreads / 32) {
         const float ref = sm[g * per].x;
-        double count = 0.0, sum = 0.0, m2 = 0.0;
         auto each = [&](auto&& fn) {
             // e = lane * per + channel, 32 at a time
             int l = int(threadIdx.x & 31) / per;
             int c = int(threadIdx.x & 31) - l * per;
             const int dl = 32 / per, dc = 32 - dl * per;
             while (l < w.lanes) {
-                const int at = l * w.cols + g * per + c;
-                const uint32_t n = cnt[at / VEC];
-                if (n > 0) fn(float(n), sm[at]);
+                const int at = l * cols + g * per + c;
+                const uint32_t n = cnt[at / runs];
+                if (n > 0) fn(float(n * d.run), sm[at]);
                 l += dl;
                 c += dc;
                 if (c >= per) {
@@ -345,22 +486,22 @@ __global__ void __launch_bounds__(kGnThreads)
                 }
             }
         };
+        float count = 0.f, sum = 0.f, all = 0.f;
         each([&](float n, float2 v) {
             count += n;
-            sum += double(n) * double(v.x - ref);
+            sum += n * (v.x - ref);
         });
         count = warp_sum(count);
-        const double off = warp_sum(sum) / count;
-        const float off32 = float(off);
+        const float off = warp_sum(sum) / count;
         each([&](float n, float2 v) {
-            const float e = v.x - ref - off32;
-            m2 += double(v.y) + double(n * e) * double(e);
+            const float e = v.x - ref - off;
+            all += v.y + n * e * e;
         });
-        m2 = warp_sum(m2);
+        all = warp_sum(all);
         if ((threadIdx.x & 31) == 0)
             part[(n * d.G + g0 + g) * d.chunks * d.pieces +
                  size_t(chunk) * d.pieces + slab % d.pieces] =
-                    make_double2(double(ref) + off, m2);
+                    make_double2(double(ref) + double(off), double(all));
     }
 }
 
@@ -416,28 +557,71 @@ __global__ void __launch_bounds__(kGnThreads)
     const uint32_t chunk = d.slabs == 1 ? i : i / uint32_t(d.slabs);
     const Walk w = walk_of<VEC>(d, chunk, slab);
     if (w.steps == 0) return;
-    float mu[VEC], a[VEC], b[VEC];
-    each_channel<VEC>(d, w, [&](int j, int c, int g) {
-        mu[j] = mean[n * d.G + g];
-        a[j] = rstd[n * d.G + g] * (weight ? weight[c] : 1.f);
-        b[j] = bias ? bias[c] : 0.f;
-    });
+    constexpr int P = kPairs<VEC>;
+    Two mu[P], a[P], b[P];
+    {
+        float m1[2 * P], a1[2 * P], b1[2 * P];
+        each_channel<VEC>(d, w, [&](int j, int c, int g) {
+            m1[j] = -mean[n * d.G + g];
+            a1[j] = rstd[n * d.G + g] * (weight ? weight[c] : 1.f);
+            b1[j] = bias ? bias[c] : 0.f;
+        });
+        if (VEC == 1) m1[1] = a1[1] = b1[1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            mu[j] = two(m1[2 * j], m1[2 * j + 1]);
+            a[j] = two(a1[2 * j], a1[2 * j + 1]);
+            b[j] = two(b1[2 * j], b1[2 * j + 1]);
+        }
+    }
     T* to = y + n * d.rows * d.C + w.base;
     walk_over<T, VEC, 1>(
             x + n * d.rows * d.C + w.base, static_cast<const T*>(nullptr),
             w.step, w.steps, ring,
-            [&](uint32_t, const Pack<T, VEC>& v, const Pack<T, VEC>&) {
-                Pack<T, VEC> o;
+            [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) {
+                Two e[P];
+                unpack<T, VEC>(v, e);
 #pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    o.v[j] = from_f<T>(act_<ACT>(
-                            (to_f<T>(v.v[j]) - mu[j]) * a[j] + b[j]));
-                *reinterpret_cast<Pack<T, VEC>*>(to) = o;
+                for (int j = 0; j < P; j++)
+                    e[j] = act2<ACT>(fma2(add2(e[j], mu[j]), a[j], b[j]));
+                *reinterpret_cast<Pack<T, VEC>*>(to) = pack<T, VEC>(e);
                 to += w.step;
             });
 }
 
 // ----------------------------------------------------------------- backward
+
+// What a thread's channels are scaled by: -mean, rstd, weight, bias.
+template <int VEC>
+struct Scales {
+    Two mu[kPairs<VEC>], r[kPairs<VEC>], wt[kPairs<VEC>], b[kPairs<VEC>];
+};
+template <int VEC>
+__device__ __forceinline__ Scales<VEC> scales_of(const GnDims& d,
+                                                 const Walk& w, uint64_t n,
+                                                 const float* weight,
+                                                 const float* bias,
+                                                 const float* mean,
+                                                 const float* rstd) {
+    constexpr int P = kPairs<VEC>;
+    float m1[2 * P], r1[2 * P], w1[2 * P], b1[2 * P];
+    each_channel<VEC>(d, w, [&](int j, int c, int g) {
+        m1[j] = -mean[n * d.G + g];
+        r1[j] = rstd[n * d.G + g];
+        w1[j] = weight ? weight[c] : 1.f;
+        b1[j] = bias ? bias[c] : 0.f;
+    });
+    if (VEC == 1) m1[1] = r1[1] = w1[1] = b1[1] = 0.f;
+    Scales<VEC> s;
+#pragma unroll
+    for (int j = 0; j < P; j++) {
+        s.mu[j] = two(m1[2 * j], m1[2 * j + 1]);
+        s.r[j] = two(r1[2 * j], r1[2 * j + 1]);
+        s.wt[j] = two(w1[2 * j], w1[2 * j + 1]);
+        s.b[j] = two(b1[2 * j], b1[2 * j + 1]);
+    }
+    return s;
+}
 
 // part[n][chunk][c] = (sum dz, sum dz h) over the chunk's rows.
 template <typename T, int VEC, int ACT>
@@ -450,37 +634,45 @@ __global__ void __launch_bounds__(kGnThreads)
                        const float* __restrict__ rstd,
                        float2* __restrict__ part) {
     extern __shared__ __align__(16) char ring[];
-    __shared__ float2 sm[kGnThreads * VEC];
     const int slab = d.slabs == 1 ? 0 : int(blockIdx.x % uint32_t(d.slabs));
     const uint32_t chunk =
             d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
     const uint64_t n = blockIdx.y;
     const Walk w = walk_of<VEC>(d, chunk, slab);
+    constexpr int P = kPairs<VEC>;
+    Two A[P], B[P];
     if (w.works) {
-        float mu[VEC], r[VEC], wt[VEC], b[VEC], A[VEC], B[VEC];
-        each_channel<VEC>(d, w, [&](int j, int c, int g) {
-            mu[j] = mean[n * d.G + g];
-            r[j] = rstd[n * d.G + g];
-            wt[j] = weight ? weight[c] : 1.f;
-            b[j] = bias ? bias[c] : 0.f;
-            A[j] = B[j] = 0.f;
-        });
+        const Scales<VEC> c =
+                scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
+#pragma unroll
+        for (int j = 0; j < P; j++) A[j] = B[j] = two(0.f);
         const uint64_t at = n * d.rows * d.C + w.base;
         walk_over<T, VEC, 2>(
                 x + at, dy + at, w.step, w.steps, ring,
-                [&](uint32_t, const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
+                [&](const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
+                    Two h[P], g[P];
+                    unpack<T, VEC>(v, h);
+                    unpack<T, VEC>(e, g);
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const float h = (to_f<T>(v.v[j]) - mu[j]) * r[j];
-                        const float dz = act_grad<ACT>(to_f<T>(e.v[j]),
-                                                       h * wt[j] + b[j]);
-                        A[j] += dz;
-                        B[j] += dz * h;
+                    for (int j = 0; j < P; j++) {
+                        h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
+                        g[j] = act_grad2<ACT>(g[j],
+                                              fma2(h[j], c.wt[j], c.b[j]));
+                        A[j] = add2(A[j], g[j]);
+                        B[j] = fma2(g[j], h[j], B[j]);
                     }
                 });
+    }
+    // the ring is free once every thread has left it
+    __syncthreads();
+    float2* const sm = reinterpret_cast<float2*>(ring);
+    if (w.works) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++)
-            sm[threadIdx.x * VEC + j] = make_float2(A[j], B[j]);
+        for (int j = 0; j < VEC; j++) {
+            const float2 a = of_two(A[j / 2]), b = of_two(B[j / 2]);
+            sm[threadIdx.x * VEC + j] =
+                    j % 2 ? make_float2(a.y, b.y) : make_float2(a.x, b.x);
+        }
     }
     __syncthreads();
     float2* out = part + (n * d.chunks + chunk) * d.C + w.col0;
@@ -566,30 +758,39 @@ __global__ void __launch_bounds__(kGnThreads)
     const uint32_t chunk = d.slabs == 1 ? i : i / uint32_t(d.slabs);
     const Walk w = walk_of<VEC>(d, chunk, slab);
     if (w.steps == 0) return;
-    float mu[VEC], r[VEC], wt[VEC], b[VEC], ma[VEC], mb[VEC];
-    each_channel<VEC>(d, w, [&](int j, int c, int g) {
-        mu[j] = mean[n * d.G + g];
-        r[j] = rstd[n * d.G + g];
-        wt[j] = weight ? weight[c] : 1.f;
-        b[j] = bias ? bias[c] : 0.f;
-        const float2 m = means[n * d.G + g];
-        ma[j] = m.x;
-        mb[j] = m.y;
-    });
+    constexpr int P = kPairs<VEC>;
+    const Scales<VEC> c = scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
+    Two ma[P], mb[P];
+    {
+        float a1[2 * P], b1[2 * P];
+        each_channel<VEC>(d, w, [&](int j, int, int g) {
+            const float2 m = means[n * d.G + g];
+            a1[j] = -m.x;
+            b1[j] = -m.y;
+        });
+        if (VEC == 1) a1[1] = b1[1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            ma[j] = two(a1[2 * j], a1[2 * j + 1]);
+            mb[j] = two(b1[2 * j], b1[2 * j + 1]);
+        }
+    }
     const uint64_t at = n * d.rows * d.C + w.base;
     T* to = dx + at;
     walk_over<T, VEC, 2>(
             x + at, dy + at, w.step, w.steps, ring,
-            [&](uint32_t, const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
-                Pack<T, VEC> o;
+            [&](const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
+                Two h[P], g[P];
+                unpack<T, VEC>(v, h);
+                unpack<T, VEC>(e, g);
 #pragma unroll
-                for (int j = 0; j < VEC; j++) {
-                    const float h = (to_f<T>(v.v[j]) - mu[j]) * r[j];
-                    const float dz =
-                            act_grad<ACT>(to_f<T>(e.v[j]), h * wt[j] + b[j]);
-                    o.v[j] = from_f<T>(r[j] * (wt[j] * dz - ma[j] - h * mb[j]));
+                for (int j = 0; j < P; j++) {
+                    h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
+                    g[j] = act_grad2<ACT>(g[j], fma2(h[j], c.wt[j], c.b[j]));
+                    g[j] = mul2(c.r[j], fma2(h[j], mb[j],
+                                             fma2(c.wt[j], g[j], ma[j])));
                 }
-                *reinterpret_cast<Pack<T, VEC>*>(to) = o;
+                *reinterpret_cast<Pack<T, VEC>*>(to) = pack<T, VEC>(g);
                 to += w.step;
             });
 }
@@ -681,11 +882,13 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
         d.threads = kGnThreads;
     }
     p.vec = vec;
+    d.run = vec;
+    while (d.cpg % d.run != 0) d.run /= 2;
     const uint64_t bytes = std::max<uint64_t>(1, sample * es * (grad ? 2 : 1));
     p.batch = std::min<uint64_t>(std::max<uint64_t>(1, kGnRoundBytes / bytes),
                                  std::min<uint64_t>(a.n, 65535));
     // one wave of resident blocks; a thread takes 4 steps or more
-    const uint64_t wave = 148 * (grad ? 3 : 4);
+    const uint64_t wave = 148 * (grad ? 2 : 4);
     uint64_t chunks = std::max<uint64_t>(
             1, wave / std::max<uint64_t>(1, p.batch * d.slabs));
     const uint64_t lanes = std::max<uint64_t>(
