@@ -50,6 +50,7 @@ struct GnDims {
     int threads;       // flat: threads that work (they cover whole rows)
     int lanes;         // flat: rows they cover
     int run;           // channels of a group that a vector holds side by side
+    int slots;         // resident: steps that a block keeps
 };
 
 template <typename T>
@@ -391,41 +392,35 @@ __device__ __forceinline__ Two act_grad2(Two dy, Two z) {
 // (the pairwise update of Chan, Golub and LeVeque, all at once). Means enter
 // as distances from one of them: of 1e4 deviations they keep no digits of the
 // variance in 32 bits.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kGnThreads)
-        k_gn_stats(GnDims d, const T* __restrict__ x,
-                   double2* __restrict__ part) {
-    extern __shared__ __align__(16) char ring[];
-    __shared__ uint32_t cnt[kGnThreads];
-    const int slab = d.slabs == 1 ? 0 : int(blockIdx.x % uint32_t(d.slabs));
-    const uint32_t chunk =
-            d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
-    const uint64_t n = blockIdx.y;
-    const Walk w = walk_of<VEC>(d, chunk, slab);
-    constexpr int P = kPairs<VEC>;
-    float mean[2 * P], m2[2 * P];
-    if (w.steps > 0) {
-        Two k[P], s1[P], s2[P];
-        const T* own = x + n * d.rows * d.C + w.base;
-        unpack<T, VEC>(load_pack<T, VEC>(own), k);
+template <int VEC>
+struct ThreadMoments {
+    static constexpr int P = kPairs<VEC>;
+    Two k[P], s1[P], s2[P];
+
+    template <typename T>
+    __device__ __forceinline__ void begin(const Pack<T, VEC>& first) {
+        unpack<T, VEC>(first, k);
 #pragma unroll
         for (int j = 0; j < P; j++) {
             k[j] = mul2(k[j], two(-1.f));
             s1[j] = s2[j] = two(0.f);
         }
-        walk_over<T, VEC, 1>(
-                own, static_cast<const T*>(nullptr), w.step, w.steps, ring,
-                [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) {
-                    Two e[P];
-                    unpack<T, VEC>(v, e);
+    }
+    template <typename T>
+    __device__ __forceinline__ void add(const Pack<T, VEC>& v) {
+        Two e[P];
+        unpack<T, VEC>(v, e);
 #pragma unroll
-                    for (int j = 0; j < P; j++) {
-                        e[j] = add2(e[j], k[j]);
-                        s1[j] = add2(s1[j], e[j]);
-                        s2[j] = fma2(e[j], e[j], s2[j]);
-                    }
-                });
-        const float inv = 1.f / float(w.steps);
+        for (int j = 0; j < P; j++) {
+            e[j] = add2(e[j], k[j]);
+            s1[j] = add2(s1[j], e[j]);
+            s2[j] = fma2(e[j], e[j], s2[j]);
+        }
+    }
+    // (mean, sum of squares) of each run of channels to sm.
+    __device__ __forceinline__ void put(uint32_t steps, int run, float2* sm) {
+        float mean[2 * P], m2[2 * P];
+        const float inv = 1.f / float(steps);
 #pragma unroll
         for (int j = 0; j < P; j++) {
             const Two m = mul2(s1[j], two(inv));
@@ -437,10 +432,10 @@ __global__ void __launch_bounds__(kGnThreads)
             m2[2 * j + 1] = nonneg(q.y);
         }
         // neighbours of a group: equal counts
-        float half = 0.5f * float(w.steps);
+        float half = 0.5f * float(steps);
 #pragma unroll
         for (int h = 1; h < VEC; h *= 2) {
-            if (h < d.run) {
+            if (h < run) {
 #pragma unroll
                 for (int j = 0; j < VEC; j += 2 * h) {
                     const float e = mean[j + h] - mean[j];
@@ -450,26 +445,26 @@ __global__ void __launch_bounds__(kGnThreads)
                 half *= 2.f;
             }
         }
-    }
-    // the ring is free once every thread has left it
-    __syncthreads();
-    float2* const sm = reinterpret_cast<float2*>(ring);
-    if (w.steps > 0) {
-        const int at = int(threadIdx.x) * (VEC / d.run);
+        sm += int(threadIdx.x) * (VEC / run);
 #pragma unroll
         for (int j = 0; j < VEC; j++)
-            if ((j & (d.run - 1)) == 0)
-                sm[at + j / d.run] = make_float2(mean[j], m2[j]);
+            if ((j & (run - 1)) == 0) sm[j / run] = make_float2(mean[j], m2[j]);
     }
-    cnt[threadIdx.x] = w.steps;
-    __syncthreads();
+};
+
+// Calls fn(g, mean, sum of squares) in one lane for each group g of the slab,
+// from what the threads have put into sm and their counts of steps.
+template <int VEC, typename F>
+__device__ __forceinline__ void merge_block(const GnDims& d, const Walk& w,
+                                            const float2* sm,
+                                            const uint32_t* cnt, F&& fn) {
     // sm[lane * cols + c] with runs for columns
     const int cols = w.cols / d.run, runs = VEC / d.run;
     const int per = d.pieces > 1 ? cols : d.cpg / d.run;
-    const int groups = d.pieces > 1 ? 1 : cols / per, g0 = w.col0 / d.cpg;
+    const int groups = d.pieces > 1 ? 1 : cols / per;
     for (int g = threadIdx.x / 32; g < groups; g += kGnThreads / 32) {
         const float ref = sm[g * per].x;
-        auto each = [&](auto&& fn) {
+        auto each = [&](auto&& add) {
             // e = lane * per + channel, 32 at a time
             int l = int(threadIdx.x & 31) / per;
             int c = int(threadIdx.x & 31) - l * per;
@@ -477,7 +472,7 @@ __global__ void __launch_bounds__(kGnThreads)
             while (l < w.lanes) {
                 const int at = l * cols + g * per + c;
                 const uint32_t n = cnt[at / runs];
-                if (n > 0) fn(float(n * d.run), sm[at]);
+                if (n > 0) add(float(n * d.run), sm[at]);
                 l += dl;
                 c += dc;
                 if (c >= per) {
@@ -499,10 +494,53 @@ __global__ void __launch_bounds__(kGnThreads)
         });
         all = warp_sum(all);
         if ((threadIdx.x & 31) == 0)
-            part[(n * d.G + g0 + g) * d.chunks * d.pieces +
-                 size_t(chunk) * d.pieces + slab % d.pieces] =
-                    make_double2(double(ref) + double(off), double(all));
+            fn(g, double(ref) + double(off), double(all));
     }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kGnThreads)
+        k_gn_stats(GnDims d, const T* __restrict__ x,
+                   double2* __restrict__ part) {
+    extern __shared__ __align__(16) char ring[];
+    __shared__ uint32_t cnt[kGnThreads];
+    const int slab = d.slabs == 1 ? 0 : int(blockIdx.x % uint32_t(d.slabs));
+    const uint32_t chunk =
+            d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
+    const uint64_t n = blockIdx.y;
+    const Walk w = walk_of<VEC>(d, chunk, slab);
+    ThreadMoments<VEC> m;
+    if (w.steps > 0) {
+        const T* own = x + n * d.rows * d.C + w.base;
+        m.begin(load_pack<T, VEC>(own));
+        walk_over<T, VEC, 1>(
+                own, static_cast<const T*>(nullptr), w.step, w.steps, ring,
+                [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) { m.add(v); });
+    }
+    // the ring is free once every thread has left it
+    __syncthreads();
+    float2* const sm = reinterpret_cast<float2*>(ring);
+    if (w.steps > 0) m.put(w.steps, d.run, sm);
+    cnt[threadIdx.x] = w.steps;
+    __syncthreads();
+    merge_block<VEC>(d, w, sm, cnt, [&](int g, double mean, double m2) {
+        part[(n * d.G + w.col0 / d.cpg + g) * d.chunks * d.pieces +
+             size_t(chunk) * d.pieces + slab % d.pieces] =
+                make_double2(mean, m2);
+    });
+}
+
+// Values of a group in part e of its d.chunks * d.pieces.
+__device__ __forceinline__ double part_count(const GnDims& d, uint32_t e) {
+    uint32_t chunk = e, piece = 0;
+    if (d.pieces > 1) {
+        chunk = e / d.pieces;
+        piece = e - chunk * d.pieces;
+    }
+    const uint64_t rows = min(d.chunk_rows, d.rows - chunk * d.chunk_rows);
+    return double(rows) *
+           (d.pieces > 1 ? min(d.slab_cols, d.cpg - int(piece) * d.slab_cols)
+                         : d.cpg);
 }
 
 // mean[n][g], rstd[n][g] from the parts; one warp each.
@@ -514,26 +552,14 @@ __global__ void k_gn_finish(GnDims d, uint32_t n,
     if (i >= uint64_t(n) * d.G) return;
     const uint32_t np = d.chunks * d.pieces;
     const double2* own = part + i * np;
-    auto count_of = [&](uint32_t e) {
-        uint32_t chunk = e, piece = 0;
-        if (d.pieces > 1) {
-            chunk = e / d.pieces;
-            piece = e - chunk * d.pieces;
-        }
-        const uint64_t rows = min(d.chunk_rows, d.rows - chunk * d.chunk_rows);
-        return double(rows) *
-               (d.pieces > 1
-                        ? min(d.slab_cols, d.cpg - int(piece) * d.slab_cols)
-                        : d.cpg);
-    };
     const double all = double(d.rows) * d.cpg;
     double sum = 0.0, m2 = 0.0;
     for (uint32_t e = threadIdx.x & 31; e < np; e += 32)
-        sum += count_of(e) * own[e].x;
+        sum += part_count(d, e) * own[e].x;
     const double mu = warp_sum(sum) / all;
     for (uint32_t e = threadIdx.x & 31; e < np; e += 32) {
         const double off = own[e].x - mu;
-        m2 += own[e].y + count_of(e) * off * off;
+        m2 += own[e].y + part_count(d, e) * off * off;
     }
     m2 = warp_sum(m2);
     if ((threadIdx.x & 31) == 0) {
@@ -587,6 +613,233 @@ __global__ void __launch_bounds__(kGnThreads)
                 *reinterpret_cast<Pack<T, VEC>*>(to) = pack<T, VEC>(e);
                 to += w.step;
             });
+}
+
+// ----------------------------------------------------------------- resident
+//
+// Images whose samples fit the shared memory of the whole GPU are read once: a
+// thread block keeps its part of a sample (an item) there from the statistics
+// to the result. The items of a sample exchange their sums through memory and
+// wait for one another, so the launch is cooperative: all its blocks run at
+// the same time. Blocks take items in order, gridDim apart; a sample has no
+// more items than there are blocks, so no block holds two of them, and what an
+// item waits for is held by blocks that wait for earlier samples at most.
+// Several blocks share an SM: while one waits, another loads or computes; and
+// a slot is refilled for the next item as soon as its own thread has used it.
+
+constexpr int kGnResident = 4;      // blocks an SM, forward
+constexpr int kGnResidentGrad = 3;  // backward
+constexpr int kGnSms = 148;
+constexpr uint32_t kGnPolls = 1u << 24;  // some seconds
+
+template <int BYTES>
+__device__ __forceinline__ void copy_vector(void* to, const void* from) {
+    if constexpr (BYTES == 16) {
+        copy_16(to, from);
+    } else if constexpr (BYTES == 4) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
+                             uint32_t(__cvta_generic_to_shared(to))),
+                     "l"(from)
+                     : "memory");
+    } else {
+        static_assert(BYTES == 2, "16, 4 or 2 bytes");
+        *static_cast<uint16_t*>(to) = *static_cast<const uint16_t*>(from);
+    }
+}
+
+struct Item {
+    uint64_t n;
+    uint32_t chunk;
+    int slab;
+};
+__device__ __forceinline__ Item item_of(const GnDims& d, uint32_t i) {
+    const uint32_t per = d.chunks * d.slabs, n = i / per, r = i - n * per;
+    Item t;
+    t.n = n;
+    t.chunk = d.slabs == 1 ? r : r / uint32_t(d.slabs);
+    t.slab = d.slabs == 1 ? 0 : int(r - t.chunk * d.slabs);
+    return t;
+}
+
+// Counts this block's item in and waits for the sample's others. Every thread
+// calls it; what each wrote before is seen by all blocks after.
+__device__ __forceinline__ void meet(uint32_t* arrived, uint32_t items,
+                                     uint32_t* status) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        atomicAdd(arrived, 1u);
+        uint32_t seen = 0, polls = 0;
+        for (;;) {
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];"
+                         : "=r"(seen)
+                         : "l"(arrived)
+                         : "memory");
+            if (seen >= items) break;
+            if (++polls == kGnPolls) {
+                if (status) atomicOr(status, kStatusWaitLimit);
+                break;
+            }
+            __nanosleep(32);
+        }
+    }
+    __syncthreads();
+}
+
+// Calls fn(g, sum of a, sum of b) in one lane for each of `groups` groups, of
+// add(g, e, &a, &b) over e = 0 .. parts - 1; all groups' lanes at once.
+template <typename A, typename F>
+__device__ __forceinline__ void sum_parts(int groups, uint32_t parts, A&& add,
+                                          F&& fn) {
+    int lanes = 32;
+    while (lanes > 1 && kGnThreads / lanes < groups) lanes /= 2;
+    const int lane = threadIdx.x & (lanes - 1);
+    for (int g0 = 0; g0 < groups; g0 += kGnThreads / lanes) {
+        const int g = g0 + threadIdx.x / lanes;
+        double a = 0.0, b = 0.0;
+        if (g < groups) {
+#pragma unroll 4
+            for (uint32_t e = lane; e < parts; e += lanes) add(g, e, &a, &b);
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            b += __shfl_xor_sync(0xffffffffu, b, o);
+        }
+        if (g < groups && lane == 0) fn(g, a, b);
+    }
+}
+
+__device__ __forceinline__ double2 load_l2(const double2* p) {
+    return __ldcg(p);
+}
+
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kGnThreads, kGnResident)
+        k_gn_resident(GnDims d, uint32_t items, const T* __restrict__ x,
+                      const float* __restrict__ weight,
+                      const float* __restrict__ bias, double2* part,
+                      uint32_t* arrived, uint32_t* status,
+                      float* __restrict__ mean, float* __restrict__ rstd,
+                      T* __restrict__ y) {
+    using V = Pack<T, VEC>;
+    constexpr int P = kPairs<VEC>;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ uint32_t cnt[kGnThreads];
+    V* const slot = reinterpret_cast<V*>(smem) + threadIdx.x;
+    float2* const sm = reinterpret_cast<float2*>(
+            smem + size_t(d.slots) * kGnThreads * sizeof(V));
+    float2* const stat = sm + kGnThreads * (VEC / d.run);
+    const uint32_t per = d.chunks * d.slabs, parts = d.chunks * d.pieces;
+
+    uint32_t i = blockIdx.x;
+    Item t = item_of(d, i);
+    Walk w = walk_of<VEC>(d, t.chunk, t.slab);
+    {
+        const T* p = x + t.n * d.rows * d.C + w.base;
+        for (uint32_t k = 0; k < w.steps; k++, p += w.step)
+            copy_vector<sizeof(V)>(slot + k * kGnThreads, p);
+    }
+    for (;;) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (w.steps > 0) {
+            ThreadMoments<VEC> m;
+            m.begin(*slot);
+            for (uint32_t k = 1; k < w.steps; k++) m.add(slot[k * kGnThreads]);
+            m.put(w.steps, d.run, sm);
+        }
+        cnt[threadIdx.x] = w.steps;
+        __syncthreads();
+        const uint64_t g0 = t.n * d.G + w.col0 / d.cpg;
+        const int groups = d.pieces > 1 ? 1 : w.cols / d.cpg;
+        const double all = double(d.rows) * d.cpg;
+        if (per == 1) {
+            merge_block<VEC>(d, w, sm, cnt, [&](int g, double mu, double m2) {
+                stat[g] = make_float2(
+                        float(mu), float(1.0 / sqrt(m2 / all + d.eps)));
+            });
+        } else {
+            merge_block<VEC>(d, w, sm, cnt, [&](int g, double mu, double m2) {
+                part[(g0 + g) * parts + size_t(t.chunk) * d.pieces +
+                     t.slab % d.pieces] = make_double2(mu, m2);
+            });
+            meet(arrived + t.n, per, status);
+            // about the first part's mean
+            sum_parts(
+                    groups, parts,
+                    [&](int g, uint32_t e, double* a, double* b) {
+                        const double2* own = part + (g0 + g) * parts;
+                        const double2 v = load_l2(own + e);
+                        const double off = v.x - load_l2(own).x;
+                        const double c = part_count(d, e);
+                        *a += c * off;
+                        *b += v.y + c * off * off;
+                    },
+                    [&](int g, double a, double b) {
+                        const double off = a / all;
+                        const double m2 = b - a * off;
+                        stat[g] = make_float2(
+                                float(load_l2(part + (g0 + g) * parts).x + off),
+                                float(1.0 / sqrt((m2 < 0.0 ? 0.0 : m2) / all +
+                                                 d.eps)));
+                    });
+        }
+        __syncthreads();
+        if (mean && t.chunk == 0 && t.slab % d.pieces == 0) {
+            for (int g = threadIdx.x; g < groups; g += kGnThreads) {
+                mean[g0 + g] = stat[g].x;
+                rstd[g0 + g] = stat[g].y;
+            }
+        }
+        Two mu[P], a[P], b[P];
+        {
+            float m1[2 * P], a1[2 * P], b1[2 * P];
+            const int first = w.col0 / d.cpg;
+            each_channel<VEC>(d, w, [&](int j, int c, int g) {
+                const float2 st = stat[g - first];
+                m1[j] = -st.x;
+                a1[j] = st.y * (weight ? weight[c] : 1.f);
+                b1[j] = bias ? bias[c] : 0.f;
+            });
+            if (VEC == 1) m1[1] = a1[1] = b1[1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+                mu[j] = two(m1[2 * j], m1[2 * j + 1]);
+                a[j] = two(a1[2 * j], a1[2 * j + 1]);
+                b[j] = two(b1[2 * j], b1[2 * j + 1]);
+            }
+        }
+        i += gridDim.x;
+        const bool more = i < items;
+        T* to = y + t.n * d.rows * d.C + w.base;
+        const uint32_t steps = w.steps;
+        const uint64_t step = w.step;
+        const T* p = nullptr;
+        if (more) {
+            t = item_of(d, i);
+            w = walk_of<VEC>(d, t.chunk, t.slab);
+            p = x + t.n * d.rows * d.C + w.base;
+        } else {
+            w.steps = 0;
+        }
+        V* at = slot;
+        for (uint32_t k = 0; k < steps; k++, at += kGnThreads, to += step) {
+            Two e[P];
+            unpack<T, VEC>(*at, e);
+            if (k < w.steps) {
+                copy_vector<sizeof(V)>(at, p);
+                p += w.step;
+            }
+#pragma unroll
+            for (int j = 0; j < P; j++)
+                e[j] = act2<ACT>(fma2(add2(e[j], mu[j]), a[j], b[j]));
+            *reinterpret_cast<V*>(to) = pack<T, VEC>(e);
+        }
+        for (uint32_t k = steps; k < w.steps; k++, at += kGnThreads) {
+            copy_vector<sizeof(V)>(at, p);
+            p += w.step;
+        }
+        if (!more) break;
+    }
 }
 
 // ----------------------------------------------------------------- backward
@@ -795,20 +1048,200 @@ __global__ void __launch_bounds__(kGnThreads)
             });
 }
 
-// dweight[c], dbias[c] = the sums over samples (in order).
-__global__ void k_gn_grad_affine(GnDims d, const float2* sums, float* dweight,
-                                 float* dbias) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= d.C) return;
-    double a = 0.0, b = 0.0;
-#pragma unroll 8
-    for (uint64_t n = 0; n < d.n; n++) {
-        const float2 v = sums[n * d.C + c];
-        a += v.x;
-        b += v.y;
+// dx and part sums of an item that stays in shared memory; sums[n][chunk][c]
+// for k_gn_grad_affine.
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
+        k_gn_resident_grad(GnDims d, uint32_t items, const T* __restrict__ dy,
+                           const T* __restrict__ x,
+                           const float* __restrict__ weight,
+                           const float* __restrict__ bias,
+                           const float* __restrict__ mean,
+                           const float* __restrict__ rstd, double2* part,
+                           uint32_t* arrived, uint32_t* status,
+                           float2* __restrict__ sums, T* __restrict__ dx) {
+    using V = Pack<T, VEC>;
+    constexpr int P = kPairs<VEC>;
+    extern __shared__ __align__(16) char smem[];
+    // x and dy of a step side by side
+    V* const slot = reinterpret_cast<V*>(smem) + threadIdx.x;
+    float2* const sm = reinterpret_cast<float2*>(
+            smem + size_t(d.slots) * 2 * kGnThreads * sizeof(V));
+    float2* const stat = sm + kGnThreads * VEC;
+    const uint32_t per = d.chunks * d.slabs, parts = d.chunks * d.pieces;
+
+    uint32_t i = blockIdx.x;
+    Item t = item_of(d, i);
+    Walk w = walk_of<VEC>(d, t.chunk, t.slab);
+    {
+        const uint64_t at = t.n * d.rows * d.C + w.base;
+        for (uint32_t k = 0; k < w.steps; k++) {
+            copy_vector<sizeof(V)>(slot + 2 * k * kGnThreads,
+                                   x + at + k * w.step);
+            copy_vector<sizeof(V)>(slot + (2 * k + 1) * kGnThreads,
+                                   dy + at + k * w.step);
+        }
     }
-    if (dbias) dbias[c] = float(a);
-    if (dweight) dweight[c] = float(b);
+    for (;;) {
+        Scales<VEC> c;
+        if (w.works) c = scales_of<VEC>(d, w, t.n, weight, bias, mean, rstd);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (w.works) {
+            Two A[P], B[P];
+#pragma unroll
+            for (int j = 0; j < P; j++) A[j] = B[j] = two(0.f);
+            for (uint32_t k = 0; k < w.steps; k++) {
+                Two h[P], g[P];
+                unpack<T, VEC>(slot[2 * k * kGnThreads], h);
+                unpack<T, VEC>(slot[(2 * k + 1) * kGnThreads], g);
+#pragma unroll
+                for (int j = 0; j < P; j++) {
+                    h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
+                    g[j] = act_grad2<ACT>(g[j], fma2(h[j], c.wt[j], c.b[j]));
+                    A[j] = add2(A[j], g[j]);
+                    B[j] = fma2(g[j], h[j], B[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const float2 a = of_two(A[j / 2]), b = of_two(B[j / 2]);
+                sm[threadIdx.x * VEC + j] =
+                        j % 2 ? make_float2(a.y, b.y) : make_float2(a.x, b.x);
+            }
+        }
+        __syncthreads();
+        float2* const out = sums + (t.n * d.chunks + t.chunk) * d.C + w.col0;
+        for (int q = threadIdx.x; q < w.cols; q += kGnThreads) {
+            float a = 0.f, b = 0.f;
+            for (int l = 0; l < w.lanes; l++) {
+                a += sm[l * w.cols + q].x;
+                b += sm[l * w.cols + q].y;
+            }
+            out[q] = make_float2(a, b);
+            // no other thread reads this column
+            const float wt = weight ? weight[w.col0 + q] : 1.f;
+            sm[q] = make_float2(a * wt, b * wt);
+        }
+        __syncthreads();
+        const uint64_t g0 = t.n * d.G + w.col0 / d.cpg;
+        const int width = d.pieces > 1 ? w.cols : d.cpg;
+        const int groups = w.cols / width;
+        const double share = 1.0 / (double(d.rows) * d.cpg);
+        sum_parts(
+                groups, width,
+                [&](int g, uint32_t e, double* a, double* b) {
+                    const float2 v = sm[g * width + e];
+                    *a += v.x;
+                    *b += v.y;
+                },
+                [&](int g, double a, double b) {
+                    if (per == 1)
+                        stat[g] = make_float2(float(a * share),
+                                              float(b * share));
+                    else
+                        part[(g0 + g) * parts + size_t(t.chunk) * d.pieces +
+                             t.slab % d.pieces] = make_double2(a, b);
+                });
+        if (per > 1) {
+            meet(arrived + t.n, per, status);
+            sum_parts(
+                    groups, parts,
+                    [&](int g, uint32_t e, double* a, double* b) {
+                        const double2 v = load_l2(part + (g0 + g) * parts + e);
+                        *a += v.x;
+                        *b += v.y;
+                    },
+                    [&](int g, double a, double b) {
+                        stat[g] = make_float2(float(a * share),
+                                              float(b * share));
+                    });
+        }
+        __syncthreads();
+        Two ma[P], mb[P];
+        {
+            float a1[2 * P], b1[2 * P];
+            const int first = w.col0 / d.cpg;
+            each_channel<VEC>(d, w, [&](int j, int, int g) {
+                const float2 m = stat[g - first];
+                a1[j] = -m.x;
+                b1[j] = -m.y;
+            });
+            if (VEC == 1) a1[1] = b1[1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+                ma[j] = two(a1[2 * j], a1[2 * j + 1]);
+                mb[j] = two(b1[2 * j], b1[2 * j + 1]);
+            }
+        }
+        i += gridDim.x;
+        const bool more = i < items;
+        T* to = dx + t.n * d.rows * d.C + w.base;
+        const uint32_t steps = w.steps;
+        const uint64_t step = w.step;
+        uint64_t from = 0;
+        if (more) {
+            t = item_of(d, i);
+            w = walk_of<VEC>(d, t.chunk, t.slab);
+            from = t.n * d.rows * d.C + w.base;
+        } else {
+            w.steps = 0;
+        }
+        V* at = slot;
+        auto refill = [&] {
+            copy_vector<sizeof(V)>(at, x + from);
+            copy_vector<sizeof(V)>(at + kGnThreads, dy + from);
+            from += w.step;
+        };
+        for (uint32_t k = 0; k < steps;
+             k++, at += 2 * kGnThreads, to += step) {
+            Two h[P], g[P];
+            unpack<T, VEC>(*at, h);
+            unpack<T, VEC>(at[kGnThreads], g);
+            if (k < w.steps) refill();
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+                h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
+                g[j] = act_grad2<ACT>(g[j], fma2(h[j], c.wt[j], c.b[j]));
+                g[j] = mul2(c.r[j],
+                            fma2(h[j], mb[j], fma2(c.wt[j], g[j], ma[j])));
+            }
+            *reinterpret_cast<V*>(to) = pack<T, VEC>(g);
+        }
+        for (uint32_t k = steps; k < w.steps; k++, at += 2 * kGnThreads)
+            refill();
+        if (!more) break;
+    }
+}
+
+// dweight[c], dbias[c] = the sums over `rows` rows of sums[row][c], in an
+// order that their number gives: 32 columns x 16 lanes a block.
+__global__ void __launch_bounds__(512)
+        k_gn_grad_affine(int C, uint64_t rows, const float2* __restrict__ sums,
+                         float* __restrict__ dweight,
+                         float* __restrict__ dbias) {
+    __shared__ double sa[16][33], sb[16][33];
+    const int lane = threadIdx.x & 31, row = threadIdx.x / 32;
+    const int c = blockIdx.x * 32 + lane;
+    double a = 0.0, b = 0.0;
+    if (c < C) {
+#pragma unroll 8
+        for (uint64_t r = row; r < rows; r += 16) {
+            const float2 v = sums[r * C + c];
+            a += v.x;
+            b += v.y;
+        }
+    }
+    sa[row][lane] = a;
+    sb[row][lane] = b;
+    __syncthreads();
+    if (row == 0 && c < C) {
+        for (int k = 1; k < 16; k++) {
+            a += sa[k][lane];
+            b += sb[k][lane];
+        }
+        if (dbias) dbias[c] = float(a);
+        if (dweight) dweight[c] = float(b);
+    }
 }
 
 // --------------------------------------------------------------------- host
@@ -817,6 +1250,8 @@ struct GnPlan {
     GnDims d;
     int vec;
     uint64_t batch;  // samples per round of launches
+    uint32_t items;  // of a resident launch; 0: rounds of launches
+    int smem;        // bytes of a resident block
 };
 
 // A round of launches covers as many samples as stay in L2 between its two
@@ -827,8 +1262,14 @@ bool aligned(const void* p, size_t a) {
     return p == nullptr || reinterpret_cast<uintptr_t>(p) % a == 0;
 }
 
+void split_rows(GnDims* d, uint64_t chunks, uint64_t row_unit) {
+    d->chunk_rows = (d->rows + chunks - 1) / chunks;
+    d->chunk_rows = (d->chunk_rows + row_unit - 1) / row_unit * row_unit;
+    d->chunks = uint32_t((d->rows + d->chunk_rows - 1) / d->chunk_rows);
+}
+
 GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
-                 bool grad) {
+                 bool grad, bool resident) {
     const int es = a.dtype == 0 ? 4 : 2;
     GnPlan p{};
     GnDims& d = p.d;
@@ -839,7 +1280,9 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     d.cpg = a.C / a.G;
     d.eps = a.eps;
     d.pieces = 1;
+    // vectors of 16 bytes, of 4 or of a value
     int vec = 16 / es;
+    auto narrower = [&] { vec = vec * es > 4 ? 4 / es : 1; };
     const uint64_t sample = a.rows * uint64_t(a.C);
     auto fits = [&](int v) {
         for (const void* q : ps)
@@ -847,20 +1290,23 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
         return true;
     };
     // flat: vectors need only the sample's size to be a multiple of them
-    while (vec > 1 && (sample % vec != 0 || !fits(vec))) vec /= 2;
-    int cover = a.C / std::gcd(a.C, vec);  // threads that cover whole rows
-    uint64_t row_unit = 1;                 // rows a chunk is a multiple of
+    while (vec > 1 && (sample % vec != 0 || !fits(vec))) narrower();
+    const int cover = a.C / std::gcd(a.C, vec);  // threads of whole rows
+    uint64_t row_unit = 1;  // rows a chunk is a multiple of
+    uint64_t lanes;         // rows a step of a block covers
     if (cover <= kGnThreads) {
         d.slabs = 1;
         d.slab_cols = a.C;
-        const uint64_t want = (sample / vec + cover - 1) / cover;
+        const uint64_t want =
+                std::max<uint64_t>(1, (sample / vec + cover - 1) / cover);
         d.threads = cover * int(std::min<uint64_t>(kGnThreads / cover,
-                                                   std::max<uint64_t>(want, 1)));
+                                                   want));
         d.lanes = int(int64_t(d.threads) * vec / a.C);
+        lanes = d.lanes;
         row_unit = vec / std::gcd(a.C, vec);
     } else {
         // slabs start at multiples of the vector in a row of such
-        for (;; vec /= 2) {
+        for (;; narrower()) {
             if (vec > 1 && a.C % vec != 0) continue;
             const int most = kGnThreads * vec;
             if (d.cpg <= most) {
@@ -880,30 +1326,61 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
             // vec = 1 always ends in one of the two
         }
         d.threads = kGnThreads;
+        lanes = std::max(1, kGnThreads / (std::min(d.slab_cols, a.C) / vec));
     }
     p.vec = vec;
     d.run = vec;
     while (d.cpg % d.run != 0) d.run /= 2;
-    const uint64_t bytes = std::max<uint64_t>(1, sample * es * (grad ? 2 : 1));
+
+    // Resident: the fewest chunks that fit the blocks' shared memory, then as
+    // many as fill whole waves of blocks; a thread takes 4 steps or more. A
+    // sample that fits one block stays in one (it then waits for nobody).
+    const int images = grad ? 2 : 1;
+    const uint64_t wave =
+            uint64_t(kGnSms) * (grad ? kGnResidentGrad : kGnResident);
+    const int groups = d.pieces > 1 ? 1 : std::min(d.slab_cols, a.C) / d.cpg;
+    const int side = kGnThreads * (grad ? vec : vec / d.run) * 8 + groups * 8;
+    const int space = (grad ? 73 : 54) << 10;
+    const int step_bytes = images * kGnThreads * vec * es;
+    d.slots = (space - side) / step_bytes;
+    const uint64_t most_rows = d.slots * lanes / row_unit * row_unit;
+    if (resident && most_rows > 0) {
+        const uint64_t least = (a.rows + most_rows - 1) / most_rows;
+        const uint64_t bound = uint64_t(d.slabs) * a.n;
+        if (least * d.slabs <= wave && least * bound < (1u << 30)) {
+            uint64_t chunks = least;
+            if (least > 1) {
+                const uint64_t waves = (least * bound + wave - 1) / wave;
+                chunks = std::max(least, waves * wave / bound);
+                chunks = std::min(chunks, wave / d.slabs);
+                chunks = std::min(chunks,
+                                  std::max(least, a.rows / (lanes * 4)));
+            }
+            split_rows(&d, chunks, row_unit);
+            p.items = uint32_t(bound * d.chunks);
+            // no more slots than a chunk takes
+            d.slots = int(std::min<uint64_t>(
+                    d.slots, (d.chunk_rows + lanes - 1) / lanes));
+            p.smem = d.slots * step_bytes + side;
+            return p;
+        }
+    }
+
+    // Rounds of launches: one wave of blocks, 4 steps or more a thread.
+    const uint64_t bytes = std::max<uint64_t>(1, sample * es * images);
     p.batch = std::min<uint64_t>(std::max<uint64_t>(1, kGnRoundBytes / bytes),
                                  std::min<uint64_t>(a.n, 65535));
-    // one wave of resident blocks; a thread takes 4 steps or more
-    const uint64_t wave = 148 * (grad ? 2 : 4);
     uint64_t chunks = std::max<uint64_t>(
-            1, wave / std::max<uint64_t>(1, p.batch * d.slabs));
-    const uint64_t lanes = std::max<uint64_t>(
-            1, uint64_t(d.threads) * vec /
-                       std::max(1, std::min(d.slab_cols, a.C)));
-    const uint64_t least = lanes * 4;  // rows
-    chunks = std::min(chunks, std::max<uint64_t>(1, a.rows / least));
-    d.chunk_rows = (a.rows + chunks - 1) / chunks;
-    d.chunk_rows = (d.chunk_rows + row_unit - 1) / row_unit * row_unit;
-    d.chunks = uint32_t((a.rows + d.chunk_rows - 1) / d.chunk_rows);
+            1, uint64_t(kGnSms) * (grad ? 2 : 4) /
+                       std::max<uint64_t>(1, p.batch * d.slabs));
+    chunks = std::min(chunks, std::max<uint64_t>(1, a.rows / (lanes * 4)));
+    split_rows(&d, chunks, row_unit);
     return p;
 }
 
 struct GnWorkspace {
-    double2* part;  // forward
+    double2* part;
+    uint32_t* arrived;
     float2* sums_part;
     float* mean;
     float* rstd;
@@ -912,20 +1389,25 @@ struct GnWorkspace {
     size_t bytes;
 };
 
-// The most that any alignment of the pointers needs.
 GnWorkspace carve(const GroupNormArgs& a, const GnPlan& p, bool grad,
                   char* base) {
     Arena ar;
     ar.base = base;
     ar.size = ~size_t(0);
     GnWorkspace w{};
-    const size_t nb = size_t(p.batch), parts = size_t(p.d.chunks);
-    if (grad) {
-        w.sums_part = ar.take<float2>(nb * parts * a.C);
+    const size_t parts = size_t(p.d.chunks) * p.d.pieces;
+    if (p.items) {
+        if (p.d.chunks * p.d.slabs > 1) {
+            w.part = ar.take<double2>(size_t(a.n) * a.G * parts);
+            w.arrived = ar.take<uint32_t>(size_t(a.n));
+        }
+        if (grad) w.sums = ar.take<float2>(size_t(a.n) * p.d.chunks * a.C);
+    } else if (grad) {
+        w.sums_part = ar.take<float2>(size_t(p.batch) * p.d.chunks * a.C);
         w.sums = ar.take<float2>(size_t(a.n) * a.C);
         w.means = ar.take<float2>(size_t(a.n) * a.G);
     } else {
-        w.part = ar.take<double2>(nb * a.G * parts * p.d.pieces);
+        w.part = ar.take<double2>(size_t(p.batch) * a.G * parts);
         w.mean = ar.take<float>(size_t(a.n) * a.G);
         w.rstd = ar.take<float>(size_t(a.n) * a.G);
     }
@@ -943,10 +1425,49 @@ void launch(void (*kernel)(P...), dim3 grid, int smem, cudaStream_t s,
     DRESSI_CUDA(cudaGetLastError());
 }
 
+// Launches a kernel whose blocks wait for one another, where they do.
+template <typename... P, typename... A>
+void launch_resident(void (*kernel)(P...), const GnPlan& p, int ctas_per_sm,
+                     const GnWorkspace& w, cudaStream_t s, A... args) {
+    const unsigned grid =
+            std::min<unsigned>(p.items, unsigned(kGnSms * ctas_per_sm));
+    DRESSI_CUDA(cudaFuncSetAttribute(
+            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(kGnThreads);
+    c.dynamicSmemBytes = size_t(p.smem);
+    c.stream = s;
+    cudaLaunchAttribute together{};
+    together.id = cudaLaunchAttributeCooperative;
+    together.val.cooperative = 1;
+    if (w.arrived) {
+        DRESSI_CUDA(cudaMemsetAsync(w.arrived, 0,
+                                    size_t(p.d.n) * sizeof(uint32_t), s));
+        c.attrs = &together;
+        c.numAttrs = 1;
+    }
+    DRESSI_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
+}
+
 template <typename T, int VEC>
 void forward_t(const GnPlan& p, const GroupNormArgs& a, const void* x,
                const float* weight, const float* bias, void* y, float* mean,
-               float* rstd, const GnWorkspace& w, cudaStream_t s) {
+               float* rstd, const GnWorkspace& w, uint32_t* status,
+               cudaStream_t s) {
+    if (p.items) {
+        launch_resident(a.act == 1   ? k_gn_resident<T, VEC, 1>
+                        : a.act == 2 ? k_gn_resident<T, VEC, 2>
+                                     : k_gn_resident<T, VEC, 0>,
+                        p, kGnResident, w, s, p.d, p.items,
+                        static_cast<const T*>(x), weight, bias, w.part,
+                        w.arrived, status, mean, rstd, static_cast<T*>(y));
+        return;
+    }
+    if (!mean) {
+        mean = w.mean;
+        rstd = w.rstd;
+    }
     const size_t sample = size_t(a.rows) * a.C;
     for (uint64_t n0 = 0; n0 < a.n; n0 += p.batch) {
         const uint64_t nb = std::min<uint64_t>(p.batch, a.n - n0);
@@ -973,7 +1494,22 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
                 const void* x, const float* weight, const float* bias,
                 const float* mean, const float* rstd, void* dx,
                 float* dweight, float* dbias, const GnWorkspace& w,
-                cudaStream_t s) {
+                uint32_t* status, cudaStream_t s) {
+    auto affine = [&](uint64_t rows) {
+        if (!dweight && !dbias) return;
+        k_gn_grad_affine<<<unsigned((a.C + 31) / 32), 512, 0, s>>>(
+                a.C, rows, w.sums, dweight, dbias);
+        DRESSI_CUDA(cudaGetLastError());
+    };
+    if (p.items) {
+        launch_resident(k_gn_resident_grad<T, VEC, ACT>, p, kGnResidentGrad, w,
+                        s, p.d, p.items, static_cast<const T*>(dy),
+                        static_cast<const T*>(x), weight, bias, mean, rstd,
+                        w.part, w.arrived, status, w.sums,
+                        static_cast<T*>(dx));
+        affine(a.n * p.d.chunks);
+        return;
+    }
     const size_t sample = size_t(a.rows) * a.C;
     const int bundle = std::min(32, std::max(1, 32 / p.d.cpg));
     const int bundles = (a.G + bundle - 1) / bundle;
@@ -996,11 +1532,7 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
                    weight, bias, mb, rb, static_cast<const float2*>(means),
                    static_cast<T*>(dx) + n0 * sample);
     }
-    if (dweight || dbias) {
-        k_gn_grad_affine<<<unsigned((a.C + 127) / 128), 128, 0, s>>>(
-                p.d, w.sums, dweight, dbias);
-        DRESSI_CUDA(cudaGetLastError());
-    }
+    affine(a.n);
 }
 
 template <typename T, int VEC>
@@ -1008,25 +1540,23 @@ void backward_t(const GnPlan& p, const GroupNormArgs& a, const void* dy,
                 const void* x, const float* weight, const float* bias,
                 const float* mean, const float* rstd, void* dx,
                 float* dweight, float* dbias, const GnWorkspace& w,
-                cudaStream_t s) {
+                uint32_t* status, cudaStream_t s) {
     auto* f = a.act == 1   ? backward_a<T, VEC, 1>
               : a.act == 2 ? backward_a<T, VEC, 2>
                            : backward_a<T, VEC, 0>;
-    f(p, a, dy, x, weight, bias, mean, rstd, dx, dweight, dbias, w, s);
+    f(p, a, dy, x, weight, bias, mean, rstd, dx, dweight, dbias, w, status, s);
 }
 
-// Calls fn.template operator()<T, VEC>() for the plan's type and width.
+// Calls fn(T(), integral constant VEC) for the plan's type and width.
 template <typename F>
 void by_type(int dtype, int vec, F&& fn) {
     if (dtype == 0) {
         if (vec == 4) fn(float(), std::integral_constant<int, 4>());
-        else if (vec == 2) fn(float(), std::integral_constant<int, 2>());
         else fn(float(), std::integral_constant<int, 1>());
         return;
     }
     auto half = [&](auto t) {
         if (vec == 8) fn(t, std::integral_constant<int, 8>());
-        else if (vec == 4) fn(t, std::integral_constant<int, 4>());
         else if (vec == 2) fn(t, std::integral_constant<int, 2>());
         else fn(t, std::integral_constant<int, 1>());
     };
@@ -1034,32 +1564,41 @@ void by_type(int dtype, int vec, F&& fn) {
     else half(__nv_bfloat16());
 }
 
+// Whether the current device has the SMs that resident plans count on.
+bool all_sms() {
+    int dev = 0, sms = 0;
+    DRESSI_CUDA(cudaGetDevice(&dev));
+    DRESSI_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount,
+                                       dev));
+    return sms >= kGnSms;
+}
+
 }  // namespace
 
 size_t group_norm_workspace(const GroupNormArgs& a, bool grad) {
     if (a.n == 0 || a.rows == 0) return 256;
-    // vectors get narrower with a pointer's alignment; the parts are most
-    // with the narrowest
+    // vectors get narrower with a pointer's alignment: the most of any
     size_t most = 256;
-    for (int align = 16; align >= 1; align /= 2) {
-        const GnPlan p = make_plan(
-                a, {reinterpret_cast<const void*>(uintptr_t(align))}, grad);
-        most = std::max(most, carve(a, p, grad, nullptr).bytes);
-    }
+    for (int align = 16; align >= 1; align /= 2)
+        for (bool resident : {false, true}) {
+            const GnPlan p = make_plan(
+                    a, {reinterpret_cast<const void*>(uintptr_t(align))}, grad,
+                    resident);
+            most = std::max(most, carve(a, p, grad, nullptr).bytes);
+        }
     return most;
 }
 
 void group_norm_op(const GroupNormArgs& a, const void* x, const float* weight,
                    const float* bias, void* y, float* mean, float* rstd,
-                   void* workspace, cudaStream_t s) {
+                   void* workspace, uint32_t* status, cudaStream_t s) {
     if (a.n == 0 || a.rows == 0) return;
-    const GnPlan p = make_plan(a, {x, y}, false);
+    const GnPlan p = make_plan(a, {x, y}, false, all_sms());
     const GnWorkspace w = carve(a, p, false, static_cast<char*>(workspace));
     ProfScope ps("group_norm", s);
     by_type(a.dtype, p.vec, [&](auto t, auto v) {
         forward_t<decltype(t), decltype(v)::value>(
-                p, a, x, weight, bias, y, mean ? mean : w.mean,
-                rstd ? rstd : w.rstd, w, s);
+                p, a, x, weight, bias, y, mean, rstd, w, status, s);
     });
 }
 
@@ -1067,19 +1606,19 @@ void group_norm_grad_op(const GroupNormArgs& a, const void* dy, const void* x,
                         const float* weight, const float* bias,
                         const float* mean, const float* rstd, void* dx,
                         float* dweight, float* dbias, void* workspace,
-                        cudaStream_t s) {
+                        uint32_t* status, cudaStream_t s) {
     if (a.n == 0 || a.rows == 0) {
         if (dweight) DRESSI_CUDA(cudaMemsetAsync(dweight, 0, 4ull * a.C, s));
         if (dbias) DRESSI_CUDA(cudaMemsetAsync(dbias, 0, 4ull * a.C, s));
         return;
     }
-    const GnPlan p = make_plan(a, {dy, x, dx}, true);
+    const GnPlan p = make_plan(a, {dy, x, dx}, true, dx && all_sms());
     const GnWorkspace w = carve(a, p, true, static_cast<char*>(workspace));
     ProfScope ps("group_norm_grad", s);
     by_type(a.dtype, p.vec, [&](auto t, auto v) {
         backward_t<decltype(t), decltype(v)::value>(
                 p, a, dy, x, weight, bias, mean, rstd, dx, dweight, dbias, w,
-                s);
+                status, s);
     });
 }
 
