@@ -57,8 +57,6 @@ extern "C" {
 #define DRESSI_STATUS_BIN_OVERFLOW 0x2u /* tile list capacity exceeded; the */
                                         /* excess went to the spill lists   */
                                         /* (results stay exact)             */
-#define DRESSI_STATUS_WAIT_LIMIT 0x8u   /* a block gave up waiting for the  */
-                                        /* others (results incomplete)      */
 
 /* ABI version of the loaded library (DRESSI_B200_ABI_VERSION). */
 int dressi_abi_version(void);
@@ -356,15 +354,12 @@ int dressi_group_norm_workspace(const dressi_group_norm_desc* d, int grad,
  * variance over a sample's rows and a group's channels. weight / bias
  * [channels] f32 or NULL (1 / 0). mean / rstd [n][groups] f32 receive the
  * statistics (both or neither NULL). Images are aligned to their element,
- * the workspace to 16 bytes; its contents do not matter, and calls that
- * overlap in time need one each. y must not overlap x. Where a sample fits the
- * GPU's shared memory the launch is cooperative (it waits until all its blocks
- * can run); status (a device word, or NULL) then gets DRESSI_STATUS_WAIT_LIMIT
- * if they lose one another. */
+ * the workspace to 16 bytes; its contents do not matter. y must not overlap
+ * x. */
 int dressi_group_norm(const dressi_group_norm_desc* d, const void* x,
                       const float* weight, const float* bias, void* y,
                       float* mean, float* rstd, void* workspace,
-                      size_t workspace_bytes, uint32_t* status, void* stream);
+                      size_t workspace_bytes, void* stream);
 
 /* The gradients for dy, from x and the statistics of the forward call. dx,
  * dweight and dbias are overwritten; each may be NULL. Repeats bit for bit. */
@@ -373,8 +368,7 @@ int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
                            const float* bias, const float* mean,
                            const float* rstd, void* dx, float* dweight,
                            float* dbias, void* workspace,
-                           size_t workspace_bytes, uint32_t* status,
-                           void* stream);
+                           size_t workspace_bytes, void* stream);
 
 /* The fewest bytes of workspace of dressi_grad_norm. */
 int dressi_grad_norm_workspace(size_t* bytes);

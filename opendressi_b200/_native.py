@@ -19,7 +19,6 @@ ABI_VERSION = 1
 OK, ERR_INVALID, ERR_CUDA, ERR_OOM, ERR_DEVICE = 0, 1, 2, 3, 4
 STATUS_INDEX_RANGE = 0x1
 STATUS_BIN_OVERFLOW = 0x2
-STATUS_WAIT_LIMIT = 0x8
 
 SLOT_PARAM, SLOT_ADAM_M, SLOT_ADAM_V, SLOT_ADAM_T = 0, 1, 2, 3
 SLOT_TARGET, SLOT_GRAD, SLOT_LOSS, SLOT_LOSS_HISTORY = 4, 5, 6, 7
@@ -240,11 +239,10 @@ SIGNATURES = {
                                               C.c_int,
                                               C.POINTER(C.c_size_t)]),
     "dressi_group_norm": (C.c_int, [C.POINTER(GroupNormDesc), _vp, _vp, _vp,
-                                    _vp, _vp, _vp, _vp, C.c_size_t, _vp,
-                                    _vp]),
+                                    _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "dressi_group_norm_grad": (C.c_int, [C.POINTER(GroupNormDesc), _vp, _vp,
                                          _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                                         _vp, C.c_size_t, _vp, _vp]),
+                                         _vp, C.c_size_t, _vp]),
     "dressi_grad_norm_workspace": (C.c_int, [C.POINTER(C.c_size_t)]),
     "dressi_grad_norm": (C.c_int, [_u32, _vp, _vp, _vp, _vp, _vp, C.c_size_t,
                                    _vp]),

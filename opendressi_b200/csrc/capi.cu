@@ -1117,7 +1117,7 @@ int dressi_group_norm_workspace(const dressi_group_norm_desc* d, int grad,
 int dressi_group_norm(const dressi_group_norm_desc* d, const void* x,
                       const float* weight, const float* bias, void* y,
                       float* mean, float* rstd, void* workspace,
-                      size_t workspace_bytes, uint32_t* status, void* stream) {
+                      size_t workspace_bytes, void* stream) {
     return guarded([&] {
         const GroupNormArgs a = group_norm_args(d);
         if (a.n == 0 || a.rows == 0) return;
@@ -1128,7 +1128,7 @@ int dressi_group_norm(const dressi_group_norm_desc* d, const void* x,
                                aligned_to(y, dtype_bytes(a.dtype)),
                        "group_norm: image not aligned to its element");
         group_norm_space(a, false, workspace, workspace_bytes);
-        group_norm_op(a, x, weight, bias, y, mean, rstd, workspace, status,
+        group_norm_op(a, x, weight, bias, y, mean, rstd, workspace,
                       as_stream(stream));
     });
 }
@@ -1138,8 +1138,7 @@ int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
                            const float* bias, const float* mean,
                            const float* rstd, void* dx, float* dweight,
                            float* dbias, void* workspace,
-                           size_t workspace_bytes, uint32_t* status,
-                           void* stream) {
+                           size_t workspace_bytes, void* stream) {
     return guarded([&] {
         const GroupNormArgs a = group_norm_args(d);
         const size_t es = dtype_bytes(a.dtype);
@@ -1152,7 +1151,7 @@ int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
         }
         if (!dx && !dweight && !dbias) return;
         group_norm_grad_op(a, dy, x, weight, bias, mean, rstd, dx, dweight,
-                           dbias, workspace, status, as_stream(stream));
+                           dbias, workspace, as_stream(stream));
     });
 }
 

@@ -36,6 +36,9 @@ namespace dressi {
 namespace {
 
 constexpr int kGnThreads = 256;
+constexpr int kGnSms = 148;
+constexpr int kGnResident = 4;      // resident blocks an SM, forward
+constexpr int kGnResidentGrad = 2;  // backward
 
 struct GnDims {
     uint64_t n, rows;
@@ -452,27 +455,42 @@ struct ThreadMoments {
     }
 };
 
+// How many lanes add up a group where all `groups` are added up at once.
+__device__ __forceinline__ int lanes_for(int groups) {
+    int lanes = 32;
+    while (lanes > 1 && kGnThreads / lanes < groups) lanes /= 2;
+    return lanes;
+}
+template <typename F>
+__device__ __forceinline__ F lane_sum(F v, int lanes) {
+    for (int o = lanes / 2; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 // Calls fn(g, mean, sum of squares) in one lane for each group g of the slab,
 // from what the threads have put into sm and their counts of steps.
 template <int VEC, typename F>
 __device__ __forceinline__ void merge_block(const GnDims& d, const Walk& w,
                                             const float2* sm,
                                             const uint32_t* cnt, F&& fn) {
-    // sm[lane * cols + c] with runs for columns
-    const int cols = w.cols / d.run, runs = VEC / d.run;
-    const int per = d.pieces > 1 ? cols : d.cpg / d.run;
-    const int groups = d.pieces > 1 ? 1 : cols / per;
-    for (int g = threadIdx.x / 32; g < groups; g += kGnThreads / 32) {
-        const float ref = sm[g * per].x;
+    // sm[lane * cols + c] with runs of 2^shift channels for columns
+    const int shift = __ffs(d.run) - 1, runs_shift = __ffs(VEC) - 1 - shift;
+    const int cols = w.cols >> shift;
+    const int per = d.pieces > 1 ? cols : d.cpg >> shift;
+    const int groups = d.pieces > 1 ? 1 : w.cols / d.cpg;
+    const int lanes = lanes_for(groups), lane = threadIdx.x & (lanes - 1);
+    // entry e = row * per + column: where a lane starts and how far it steps
+    const int l0 = lane / per, c0 = lane - l0 * per;
+    const int dl = lanes / per, dc = lanes - dl * per;
+    for (int b = 0; b < groups; b += kGnThreads / lanes) {
+        const int g = b + threadIdx.x / lanes;
         auto each = [&](auto&& add) {
-            // e = lane * per + channel, 32 at a time
-            int l = int(threadIdx.x & 31) / per;
-            int c = int(threadIdx.x & 31) - l * per;
-            const int dl = 32 / per, dc = 32 - dl * per;
+            int l = g < groups ? l0 : w.lanes, c = c0;
             while (l < w.lanes) {
                 const int at = l * cols + g * per + c;
-                const uint32_t n = cnt[at / runs];
-                if (n > 0) add(float(n * d.run), sm[at]);
+                const uint32_t n = cnt[at >> runs_shift];
+                if (n > 0) add(float(n << shift), sm[at]);
                 l += dl;
                 c += dc;
                 if (c >= per) {
@@ -481,19 +499,19 @@ __device__ __forceinline__ void merge_block(const GnDims& d, const Walk& w,
                 }
             }
         };
+        const float ref = g < groups ? sm[g * per].x : 0.f;
         float count = 0.f, sum = 0.f, all = 0.f;
         each([&](float n, float2 v) {
             count += n;
             sum += n * (v.x - ref);
         });
-        count = warp_sum(count);
-        const float off = warp_sum(sum) / count;
+        const float off = lane_sum(sum, lanes) / lane_sum(count, lanes);
         each([&](float n, float2 v) {
             const float e = v.x - ref - off;
             all += v.y + n * e * e;
         });
-        all = warp_sum(all);
-        if ((threadIdx.x & 31) == 0)
+        all = lane_sum(all, lanes);
+        if (g < groups && lane == 0)
             fn(g, double(ref) + double(off), double(all));
     }
 }
@@ -617,20 +635,13 @@ __global__ void __launch_bounds__(kGnThreads)
 
 // ----------------------------------------------------------------- resident
 //
-// Images whose samples fit the shared memory of the whole GPU are read once: a
-// thread block keeps its part of a sample (an item) there from the statistics
-// to the result. The items of a sample exchange their sums through memory and
-// wait for one another, so the launch is cooperative: all its blocks run at
-// the same time. Blocks take items in order, gridDim apart; a sample has no
-// more items than there are blocks, so no block holds two of them, and what an
-// item waits for is held by blocks that wait for earlier samples at most.
-// Several blocks share an SM: while one waits, another loads or computes; and
-// a slot is refilled for the next item as soon as its own thread has used it.
-
-constexpr int kGnResident = 4;      // blocks an SM, forward
-constexpr int kGnResidentGrad = 3;  // backward
-constexpr int kGnSms = 148;
-constexpr uint32_t kGnPolls = 1u << 24;  // some seconds
+// A slab of a sample that fits a block's shared memory (an item) stays there
+// from the statistics to the result: one launch, one read, no exchange. Slots
+// are each thread's own, and refilled for the block's next item as soon as the
+// thread has used them. (Keeping larger samples in several blocks that exchange
+// their sums and wait for one another was no faster than separate launches: 71
+// us against 51 for 8x256x256x64 bf16, the sums' way through memory being 8 us
+// of it each time.)
 
 template <int BYTES>
 __device__ __forceinline__ void copy_vector(void* to, const void* from) {
@@ -647,78 +658,28 @@ __device__ __forceinline__ void copy_vector(void* to, const void* from) {
     }
 }
 
-struct Item {
-    uint64_t n;
-    uint32_t chunk;
-    int slab;
-};
-__device__ __forceinline__ Item item_of(const GnDims& d, uint32_t i) {
-    const uint32_t per = d.chunks * d.slabs, n = i / per, r = i - n * per;
-    Item t;
-    t.n = n;
-    t.chunk = d.slabs == 1 ? r : r / uint32_t(d.slabs);
-    t.slab = d.slabs == 1 ? 0 : int(r - t.chunk * d.slabs);
-    return t;
-}
-
-// Counts this block's item in and waits for the sample's others. Every thread
-// calls it; what each wrote before is seen by all blocks after.
-__device__ __forceinline__ void meet(uint32_t* arrived, uint32_t items,
-                                     uint32_t* status) {
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(arrived, 1u);
-        uint32_t seen = 0, polls = 0;
-        for (;;) {
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];"
-                         : "=r"(seen)
-                         : "l"(arrived)
-                         : "memory");
-            if (seen >= items) break;
-            if (++polls == kGnPolls) {
-                if (status) atomicOr(status, kStatusWaitLimit);
-                break;
-            }
-            __nanosleep(32);
-        }
-    }
-    __syncthreads();
-}
-
 // Calls fn(g, sum of a, sum of b) in one lane for each of `groups` groups, of
 // add(g, e, &a, &b) over e = 0 .. parts - 1; all groups' lanes at once.
 template <typename A, typename F>
 __device__ __forceinline__ void sum_parts(int groups, uint32_t parts, A&& add,
                                           F&& fn) {
-    int lanes = 32;
-    while (lanes > 1 && kGnThreads / lanes < groups) lanes /= 2;
-    const int lane = threadIdx.x & (lanes - 1);
+    const int lanes = lanes_for(groups), lane = threadIdx.x & (lanes - 1);
     for (int g0 = 0; g0 < groups; g0 += kGnThreads / lanes) {
         const int g = g0 + threadIdx.x / lanes;
         double a = 0.0, b = 0.0;
-        if (g < groups) {
-#pragma unroll 4
+        if (g < groups)
             for (uint32_t e = lane; e < parts; e += lanes) add(g, e, &a, &b);
-        }
-        for (int o = lanes / 2; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
-        }
+        a = lane_sum(a, lanes);
+        b = lane_sum(b, lanes);
         if (g < groups && lane == 0) fn(g, a, b);
     }
-}
-
-__device__ __forceinline__ double2 load_l2(const double2* p) {
-    return __ldcg(p);
 }
 
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(kGnThreads, kGnResident)
         k_gn_resident(GnDims d, uint32_t items, const T* __restrict__ x,
                       const float* __restrict__ weight,
-                      const float* __restrict__ bias, double2* part,
-                      uint32_t* arrived, uint32_t* status,
+                      const float* __restrict__ bias,
                       float* __restrict__ mean, float* __restrict__ rstd,
                       T* __restrict__ y) {
     using V = Pack<T, VEC>;
@@ -729,13 +690,12 @@ __global__ void __launch_bounds__(kGnThreads, kGnResident)
     float2* const sm = reinterpret_cast<float2*>(
             smem + size_t(d.slots) * kGnThreads * sizeof(V));
     float2* const stat = sm + kGnThreads * (VEC / d.run);
-    const uint32_t per = d.chunks * d.slabs, parts = d.chunks * d.pieces;
 
     uint32_t i = blockIdx.x;
-    Item t = item_of(d, i);
-    Walk w = walk_of<VEC>(d, t.chunk, t.slab);
+    uint64_t n = i / uint32_t(d.slabs);
+    Walk w = walk_of<VEC>(d, 0, int(i % uint32_t(d.slabs)));
     {
-        const T* p = x + t.n * d.rows * d.C + w.base;
+        const T* p = x + n * d.rows * d.C + w.base;
         for (uint32_t k = 0; k < w.steps; k++, p += w.step)
             copy_vector<sizeof(V)>(slot + k * kGnThreads, p);
     }
@@ -749,51 +709,21 @@ __global__ void __launch_bounds__(kGnThreads, kGnResident)
         }
         cnt[threadIdx.x] = w.steps;
         __syncthreads();
-        const uint64_t g0 = t.n * d.G + w.col0 / d.cpg;
-        const int groups = d.pieces > 1 ? 1 : w.cols / d.cpg;
+        const int first = w.col0 / d.cpg, groups = w.cols / d.cpg;
         const double all = double(d.rows) * d.cpg;
-        if (per == 1) {
-            merge_block<VEC>(d, w, sm, cnt, [&](int g, double mu, double m2) {
-                stat[g] = make_float2(
-                        float(mu), float(1.0 / sqrt(m2 / all + d.eps)));
-            });
-        } else {
-            merge_block<VEC>(d, w, sm, cnt, [&](int g, double mu, double m2) {
-                part[(g0 + g) * parts + size_t(t.chunk) * d.pieces +
-                     t.slab % d.pieces] = make_double2(mu, m2);
-            });
-            meet(arrived + t.n, per, status);
-            // about the first part's mean
-            sum_parts(
-                    groups, parts,
-                    [&](int g, uint32_t e, double* a, double* b) {
-                        const double2* own = part + (g0 + g) * parts;
-                        const double2 v = load_l2(own + e);
-                        const double off = v.x - load_l2(own).x;
-                        const double c = part_count(d, e);
-                        *a += c * off;
-                        *b += v.y + c * off * off;
-                    },
-                    [&](int g, double a, double b) {
-                        const double off = a / all;
-                        const double m2 = b - a * off;
-                        stat[g] = make_float2(
-                                float(load_l2(part + (g0 + g) * parts).x + off),
-                                float(1.0 / sqrt((m2 < 0.0 ? 0.0 : m2) / all +
-                                                 d.eps)));
-                    });
-        }
-        __syncthreads();
-        if (mean && t.chunk == 0 && t.slab % d.pieces == 0) {
-            for (int g = threadIdx.x; g < groups; g += kGnThreads) {
-                mean[g0 + g] = stat[g].x;
-                rstd[g0 + g] = stat[g].y;
+        merge_block<VEC>(d, w, sm, cnt, [&](int g, double mu, double m2) {
+            const float2 st = make_float2(
+                    float(mu), float(1.0 / sqrt(m2 / all + d.eps)));
+            stat[g] = st;
+            if (mean) {
+                mean[n * d.G + first + g] = st.x;
+                rstd[n * d.G + first + g] = st.y;
             }
-        }
+        });
+        __syncthreads();
         Two mu[P], a[P], b[P];
         {
             float m1[2 * P], a1[2 * P], b1[2 * P];
-            const int first = w.col0 / d.cpg;
             each_channel<VEC>(d, w, [&](int j, int c, int g) {
                 const float2 st = stat[g - first];
                 m1[j] = -st.x;
@@ -810,14 +740,14 @@ __global__ void __launch_bounds__(kGnThreads, kGnResident)
         }
         i += gridDim.x;
         const bool more = i < items;
-        T* to = y + t.n * d.rows * d.C + w.base;
+        T* to = y + n * d.rows * d.C + w.base;
         const uint32_t steps = w.steps;
         const uint64_t step = w.step;
         const T* p = nullptr;
         if (more) {
-            t = item_of(d, i);
-            w = walk_of<VEC>(d, t.chunk, t.slab);
-            p = x + t.n * d.rows * d.C + w.base;
+            n = i / uint32_t(d.slabs);
+            w = walk_of<VEC>(d, 0, int(i % uint32_t(d.slabs)));
+            p = x + n * d.rows * d.C + w.base;
         } else {
             w.steps = 0;
         }
@@ -1048,8 +978,8 @@ __global__ void __launch_bounds__(kGnThreads)
             });
 }
 
-// dx and part sums of an item that stays in shared memory; sums[n][chunk][c]
-// for k_gn_grad_affine.
+// dx of an item that stays in shared memory, and sums[n][c] = (sum dz,
+// sum dz h).
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
         k_gn_resident_grad(GnDims d, uint32_t items, const T* __restrict__ dy,
@@ -1057,8 +987,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
                            const float* __restrict__ weight,
                            const float* __restrict__ bias,
                            const float* __restrict__ mean,
-                           const float* __restrict__ rstd, double2* part,
-                           uint32_t* arrived, uint32_t* status,
+                           const float* __restrict__ rstd,
                            float2* __restrict__ sums, T* __restrict__ dx) {
     using V = Pack<T, VEC>;
     constexpr int P = kPairs<VEC>;
@@ -1068,13 +997,12 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
     float2* const sm = reinterpret_cast<float2*>(
             smem + size_t(d.slots) * 2 * kGnThreads * sizeof(V));
     float2* const stat = sm + kGnThreads * VEC;
-    const uint32_t per = d.chunks * d.slabs, parts = d.chunks * d.pieces;
 
     uint32_t i = blockIdx.x;
-    Item t = item_of(d, i);
-    Walk w = walk_of<VEC>(d, t.chunk, t.slab);
+    uint64_t n = i / uint32_t(d.slabs);
+    Walk w = walk_of<VEC>(d, 0, int(i % uint32_t(d.slabs)));
     {
-        const uint64_t at = t.n * d.rows * d.C + w.base;
+        const uint64_t at = n * d.rows * d.C + w.base;
         for (uint32_t k = 0; k < w.steps; k++) {
             copy_vector<sizeof(V)>(slot + 2 * k * kGnThreads,
                                    x + at + k * w.step);
@@ -1084,7 +1012,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
     }
     for (;;) {
         Scales<VEC> c;
-        if (w.works) c = scales_of<VEC>(d, w, t.n, weight, bias, mean, rstd);
+        if (w.works) c = scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (w.works) {
             Two A[P], B[P];
@@ -1110,57 +1038,34 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
             }
         }
         __syncthreads();
-        float2* const out = sums + (t.n * d.chunks + t.chunk) * d.C + w.col0;
         for (int q = threadIdx.x; q < w.cols; q += kGnThreads) {
-            float a = 0.f, b = 0.f;
+            double a = 0.0, b = 0.0;
             for (int l = 0; l < w.lanes; l++) {
                 a += sm[l * w.cols + q].x;
                 b += sm[l * w.cols + q].y;
             }
-            out[q] = make_float2(a, b);
+            sums[n * d.C + w.col0 + q] = make_float2(float(a), float(b));
             // no other thread reads this column
-            const float wt = weight ? weight[w.col0 + q] : 1.f;
-            sm[q] = make_float2(a * wt, b * wt);
+            const double wt = weight ? weight[w.col0 + q] : 1.f;
+            sm[q] = make_float2(float(a * wt), float(b * wt));
         }
         __syncthreads();
-        const uint64_t g0 = t.n * d.G + w.col0 / d.cpg;
-        const int width = d.pieces > 1 ? w.cols : d.cpg;
-        const int groups = w.cols / width;
+        const int first = w.col0 / d.cpg;
         const double share = 1.0 / (double(d.rows) * d.cpg);
         sum_parts(
-                groups, width,
+                w.cols / d.cpg, d.cpg,
                 [&](int g, uint32_t e, double* a, double* b) {
-                    const float2 v = sm[g * width + e];
+                    const float2 v = sm[g * d.cpg + e];
                     *a += v.x;
                     *b += v.y;
                 },
                 [&](int g, double a, double b) {
-                    if (per == 1)
-                        stat[g] = make_float2(float(a * share),
-                                              float(b * share));
-                    else
-                        part[(g0 + g) * parts + size_t(t.chunk) * d.pieces +
-                             t.slab % d.pieces] = make_double2(a, b);
+                    stat[g] = make_float2(float(a * share), float(b * share));
                 });
-        if (per > 1) {
-            meet(arrived + t.n, per, status);
-            sum_parts(
-                    groups, parts,
-                    [&](int g, uint32_t e, double* a, double* b) {
-                        const double2 v = load_l2(part + (g0 + g) * parts + e);
-                        *a += v.x;
-                        *b += v.y;
-                    },
-                    [&](int g, double a, double b) {
-                        stat[g] = make_float2(float(a * share),
-                                              float(b * share));
-                    });
-        }
         __syncthreads();
         Two ma[P], mb[P];
         {
             float a1[2 * P], b1[2 * P];
-            const int first = w.col0 / d.cpg;
             each_channel<VEC>(d, w, [&](int j, int, int g) {
                 const float2 m = stat[g - first];
                 a1[j] = -m.x;
@@ -1175,14 +1080,14 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
         }
         i += gridDim.x;
         const bool more = i < items;
-        T* to = dx + t.n * d.rows * d.C + w.base;
+        T* to = dx + n * d.rows * d.C + w.base;
         const uint32_t steps = w.steps;
         const uint64_t step = w.step;
         uint64_t from = 0;
         if (more) {
-            t = item_of(d, i);
-            w = walk_of<VEC>(d, t.chunk, t.slab);
-            from = t.n * d.rows * d.C + w.base;
+            n = i / uint32_t(d.slabs);
+            w = walk_of<VEC>(d, 0, int(i % uint32_t(d.slabs)));
+            from = n * d.rows * d.C + w.base;
         } else {
             w.steps = 0;
         }
@@ -1251,6 +1156,7 @@ struct GnPlan {
     int vec;
     uint64_t batch;  // samples per round of launches
     uint32_t items;  // of a resident launch; 0: rounds of launches
+    uint32_t grid;   // its blocks
     int smem;        // bytes of a resident block
 };
 
@@ -1332,36 +1238,26 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     d.run = vec;
     while (d.cpg % d.run != 0) d.run /= 2;
 
-    // Resident: the fewest chunks that fit the blocks' shared memory, then as
-    // many as fill whole waves of blocks; a thread takes 4 steps or more. A
-    // sample that fits one block stays in one (it then waits for nobody).
+    // Resident: a slab of a sample in one block, several blocks an SM where
+    // there are that many.
     const int images = grad ? 2 : 1;
-    const uint64_t wave =
-            uint64_t(kGnSms) * (grad ? kGnResidentGrad : kGnResident);
-    const int groups = d.pieces > 1 ? 1 : std::min(d.slab_cols, a.C) / d.cpg;
+    const uint64_t items = uint64_t(d.slabs) * a.n;
+    const int groups = std::min(d.slab_cols, a.C) / d.cpg;
     const int side = kGnThreads * (grad ? vec : vec / d.run) * 8 + groups * 8;
-    const int space = (grad ? 73 : 54) << 10;
     const int step_bytes = images * kGnThreads * vec * es;
-    d.slots = (space - side) / step_bytes;
-    const uint64_t most_rows = d.slots * lanes / row_unit * row_unit;
-    if (resident && most_rows > 0) {
-        const uint64_t least = (a.rows + most_rows - 1) / most_rows;
-        const uint64_t bound = uint64_t(d.slabs) * a.n;
-        if (least * d.slabs <= wave && least * bound < (1u << 30)) {
-            uint64_t chunks = least;
-            if (least > 1) {
-                const uint64_t waves = (least * bound + wave - 1) / wave;
-                chunks = std::max(least, waves * wave / bound);
-                chunks = std::min(chunks, wave / d.slabs);
-                chunks = std::min(chunks,
-                                  std::max(least, a.rows / (lanes * 4)));
-            }
-            split_rows(&d, chunks, row_unit);
-            p.items = uint32_t(bound * d.chunks);
-            // no more slots than a chunk takes
-            d.slots = int(std::min<uint64_t>(
-                    d.slots, (d.chunk_rows + lanes - 1) / lanes));
-            p.smem = d.slots * step_bytes + side;
+    const uint64_t steps = (a.rows + lanes - 1) / lanes;
+    const int most = grad ? kGnResidentGrad : kGnResident;
+    if (resident && d.pieces == 1 && items < (1u << 30)) {
+        for (int each = most; each >= 1; each /= 2) {
+            const uint64_t bytes = steps * step_bytes + side;
+            if (bytes > uint64_t(226 / each - 3) << 10) continue;
+            if (each < most && items > uint64_t(kGnSms) * each) break;
+            split_rows(&d, 1, row_unit);
+            d.slots = int(steps);
+            p.items = uint32_t(items);
+            p.grid = uint32_t(
+                    std::min<uint64_t>(items, uint64_t(kGnSms) * each));
+            p.smem = int(bytes);
             return p;
         }
     }
@@ -1380,7 +1276,6 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
 
 struct GnWorkspace {
     double2* part;
-    uint32_t* arrived;
     float2* sums_part;
     float* mean;
     float* rstd;
@@ -1397,11 +1292,7 @@ GnWorkspace carve(const GroupNormArgs& a, const GnPlan& p, bool grad,
     GnWorkspace w{};
     const size_t parts = size_t(p.d.chunks) * p.d.pieces;
     if (p.items) {
-        if (p.d.chunks * p.d.slabs > 1) {
-            w.part = ar.take<double2>(size_t(a.n) * a.G * parts);
-            w.arrived = ar.take<uint32_t>(size_t(a.n));
-        }
-        if (grad) w.sums = ar.take<float2>(size_t(a.n) * p.d.chunks * a.C);
+        if (grad) w.sums = ar.take<float2>(size_t(a.n) * a.C);
     } else if (grad) {
         w.sums_part = ar.take<float2>(size_t(p.batch) * p.d.chunks * a.C);
         w.sums = ar.take<float2>(size_t(a.n) * a.C);
@@ -1425,43 +1316,17 @@ void launch(void (*kernel)(P...), dim3 grid, int smem, cudaStream_t s,
     DRESSI_CUDA(cudaGetLastError());
 }
 
-// Launches a kernel whose blocks wait for one another, where they do.
-template <typename... P, typename... A>
-void launch_resident(void (*kernel)(P...), const GnPlan& p, int ctas_per_sm,
-                     const GnWorkspace& w, cudaStream_t s, A... args) {
-    const unsigned grid =
-            std::min<unsigned>(p.items, unsigned(kGnSms * ctas_per_sm));
-    DRESSI_CUDA(cudaFuncSetAttribute(
-            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(grid);
-    c.blockDim = dim3(kGnThreads);
-    c.dynamicSmemBytes = size_t(p.smem);
-    c.stream = s;
-    cudaLaunchAttribute together{};
-    together.id = cudaLaunchAttributeCooperative;
-    together.val.cooperative = 1;
-    if (w.arrived) {
-        DRESSI_CUDA(cudaMemsetAsync(w.arrived, 0,
-                                    size_t(p.d.n) * sizeof(uint32_t), s));
-        c.attrs = &together;
-        c.numAttrs = 1;
-    }
-    DRESSI_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
-}
-
 template <typename T, int VEC>
 void forward_t(const GnPlan& p, const GroupNormArgs& a, const void* x,
                const float* weight, const float* bias, void* y, float* mean,
-               float* rstd, const GnWorkspace& w, uint32_t* status,
-               cudaStream_t s) {
+               float* rstd, const GnWorkspace& w, cudaStream_t s) {
     if (p.items) {
-        launch_resident(a.act == 1   ? k_gn_resident<T, VEC, 1>
-                        : a.act == 2 ? k_gn_resident<T, VEC, 2>
-                                     : k_gn_resident<T, VEC, 0>,
-                        p, kGnResident, w, s, p.d, p.items,
-                        static_cast<const T*>(x), weight, bias, w.part,
-                        w.arrived, status, mean, rstd, static_cast<T*>(y));
+        launch(a.act == 1   ? k_gn_resident<T, VEC, 1>
+               : a.act == 2 ? k_gn_resident<T, VEC, 2>
+                            : k_gn_resident<T, VEC, 0>,
+               dim3(p.grid), p.smem, s, p.d, p.items,
+               static_cast<const T*>(x), weight, bias, mean, rstd,
+               static_cast<T*>(y));
         return;
     }
     if (!mean) {
@@ -1494,7 +1359,7 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
                 const void* x, const float* weight, const float* bias,
                 const float* mean, const float* rstd, void* dx,
                 float* dweight, float* dbias, const GnWorkspace& w,
-                uint32_t* status, cudaStream_t s) {
+                cudaStream_t s) {
     auto affine = [&](uint64_t rows) {
         if (!dweight && !dbias) return;
         k_gn_grad_affine<<<unsigned((a.C + 31) / 32), 512, 0, s>>>(
@@ -1502,12 +1367,10 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
         DRESSI_CUDA(cudaGetLastError());
     };
     if (p.items) {
-        launch_resident(k_gn_resident_grad<T, VEC, ACT>, p, kGnResidentGrad, w,
-                        s, p.d, p.items, static_cast<const T*>(dy),
-                        static_cast<const T*>(x), weight, bias, mean, rstd,
-                        w.part, w.arrived, status, w.sums,
-                        static_cast<T*>(dx));
-        affine(a.n * p.d.chunks);
+        launch(k_gn_resident_grad<T, VEC, ACT>, dim3(p.grid), p.smem, s, p.d,
+               p.items, static_cast<const T*>(dy), static_cast<const T*>(x),
+               weight, bias, mean, rstd, w.sums, static_cast<T*>(dx));
+        affine(a.n);
         return;
     }
     const size_t sample = size_t(a.rows) * a.C;
@@ -1540,11 +1403,11 @@ void backward_t(const GnPlan& p, const GroupNormArgs& a, const void* dy,
                 const void* x, const float* weight, const float* bias,
                 const float* mean, const float* rstd, void* dx,
                 float* dweight, float* dbias, const GnWorkspace& w,
-                uint32_t* status, cudaStream_t s) {
+                cudaStream_t s) {
     auto* f = a.act == 1   ? backward_a<T, VEC, 1>
               : a.act == 2 ? backward_a<T, VEC, 2>
                            : backward_a<T, VEC, 0>;
-    f(p, a, dy, x, weight, bias, mean, rstd, dx, dweight, dbias, w, status, s);
+    f(p, a, dy, x, weight, bias, mean, rstd, dx, dweight, dbias, w, s);
 }
 
 // Calls fn(T(), integral constant VEC) for the plan's type and width.
@@ -1562,15 +1425,6 @@ void by_type(int dtype, int vec, F&& fn) {
     };
     if (dtype == 1) half(__half());
     else half(__nv_bfloat16());
-}
-
-// Whether the current device has the SMs that resident plans count on.
-bool all_sms() {
-    int dev = 0, sms = 0;
-    DRESSI_CUDA(cudaGetDevice(&dev));
-    DRESSI_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount,
-                                       dev));
-    return sms >= kGnSms;
 }
 
 }  // namespace
@@ -1591,14 +1445,14 @@ size_t group_norm_workspace(const GroupNormArgs& a, bool grad) {
 
 void group_norm_op(const GroupNormArgs& a, const void* x, const float* weight,
                    const float* bias, void* y, float* mean, float* rstd,
-                   void* workspace, uint32_t* status, cudaStream_t s) {
+                   void* workspace, cudaStream_t s) {
     if (a.n == 0 || a.rows == 0) return;
-    const GnPlan p = make_plan(a, {x, y}, false, all_sms());
+    const GnPlan p = make_plan(a, {x, y}, false, true);
     const GnWorkspace w = carve(a, p, false, static_cast<char*>(workspace));
     ProfScope ps("group_norm", s);
     by_type(a.dtype, p.vec, [&](auto t, auto v) {
         forward_t<decltype(t), decltype(v)::value>(
-                p, a, x, weight, bias, y, mean, rstd, w, status, s);
+                p, a, x, weight, bias, y, mean, rstd, w, s);
     });
 }
 
@@ -1606,19 +1460,19 @@ void group_norm_grad_op(const GroupNormArgs& a, const void* dy, const void* x,
                         const float* weight, const float* bias,
                         const float* mean, const float* rstd, void* dx,
                         float* dweight, float* dbias, void* workspace,
-                        uint32_t* status, cudaStream_t s) {
+                        cudaStream_t s) {
     if (a.n == 0 || a.rows == 0) {
         if (dweight) DRESSI_CUDA(cudaMemsetAsync(dweight, 0, 4ull * a.C, s));
         if (dbias) DRESSI_CUDA(cudaMemsetAsync(dbias, 0, 4ull * a.C, s));
         return;
     }
-    const GnPlan p = make_plan(a, {dy, x, dx}, true, dx && all_sms());
+    const GnPlan p = make_plan(a, {dy, x, dx}, true, dx != nullptr);
     const GnWorkspace w = carve(a, p, true, static_cast<char*>(workspace));
     ProfScope ps("group_norm_grad", s);
     by_type(a.dtype, p.vec, [&](auto t, auto v) {
         backward_t<decltype(t), decltype(v)::value>(
                 p, a, dy, x, weight, bias, mean, rstd, dx, dweight, dbias, w,
-                status, s);
+                s);
     });
 }
 

@@ -629,8 +629,6 @@ void interpolate_grad_op(const float* gy, int n_comp, int n_verts,
                          uint32_t* status, cudaStream_t s);
 
 // --- group normalisation (group_norm.cu) ---
-// DRESSI_STATUS_WAIT_LIMIT of the status word
-constexpr uint32_t kStatusWaitLimit = 0x8u;
 struct GroupNormArgs {
     uint64_t n, rows;  // x [n][rows][C]
     int C, G;
@@ -641,16 +639,15 @@ struct GroupNormArgs {
 // Bytes of workspace that a forward (grad: backward) call needs.
 size_t group_norm_workspace(const GroupNormArgs& a, bool grad);
 // y = act(group_norm(x)); mean / rstd [n][G] are written where not null.
-// status (may be null): see kStatusWaitLimit.
 void group_norm_op(const GroupNormArgs& a, const void* x, const float* weight,
                    const float* bias, void* y, float* mean, float* rstd,
-                   void* workspace, uint32_t* status, cudaStream_t s);
+                   void* workspace, cudaStream_t s);
 // dx, dweight, dbias: each may be null.
 void group_norm_grad_op(const GroupNormArgs& a, const void* dy, const void* x,
                         const float* weight, const float* bias,
                         const float* mean, const float* rstd, void* dx,
                         float* dweight, float* dbias, void* workspace,
-                        uint32_t* status, cudaStream_t s);
+                        cudaStream_t s);
 
 // --- AdamW over many tensors, norm over many tensors (adamw.cu) ---
 struct AdamWArgs {

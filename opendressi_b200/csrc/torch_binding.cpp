@@ -76,11 +76,6 @@ const float* floats(const Tensor& t) {
                        : nullptr;
 }
 
-uint32_t* word(const optional<Tensor>& status) {
-    return status ? static_cast<uint32_t*>(status->mutable_data_ptr())
-                  : nullptr;
-}
-
 // --------------------------------------------------------------- group norm
 
 Tensor table(const Tensor& t, const char* name, const Tensor& x) {
@@ -129,8 +124,7 @@ dressi_group_norm_desc norm_desc(const Tensor& x, int64_t groups, double eps,
 // y and, with stats, mean and rstd [N, groups].
 std::vector<Tensor> norm_forward(const Tensor& x_, int64_t groups,
                                  const Tensor& weight_, const Tensor& bias_,
-                                 double eps, int activation, bool stats,
-                                 const optional<Tensor>& status) {
+                                 double eps, int activation, bool stats) {
     const dressi_group_norm_desc d = norm_desc(x_, groups, eps, activation);
     const Tensor x = x_.contiguous();
     const Tensor weight = table(weight_, "weight", x);
@@ -151,8 +145,7 @@ std::vector<Tensor> norm_forward(const Tensor& x_, int64_t groups,
                            floats(bias), y.mutable_data_ptr(),
                            const_cast<float*>(floats(mean)),
                            const_cast<float*>(floats(rstd)),
-                           space.mutable_data_ptr(), need, word(status),
-                           stream_of(x)),
+                           space.mutable_data_ptr(), need, stream_of(x)),
          "group_norm");
     return {y, mean, rstd};
 }
@@ -163,8 +156,7 @@ std::vector<Tensor> norm_backward(const Tensor& dy_, const Tensor& x_,
                                   const Tensor& bias_, const Tensor& mean_,
                                   const Tensor& rstd_, double eps,
                                   int activation, bool want_x,
-                                  bool want_weight, bool want_bias,
-                                  const optional<Tensor>& status) {
+                                  bool want_weight, bool want_bias) {
     const dressi_group_norm_desc d = norm_desc(x_, groups, eps, activation);
     on_cuda(dy_, "dy");
     if (dy_.sizes() != x_.sizes() || dy_.scalar_type() != x_.scalar_type() ||
@@ -197,7 +189,7 @@ std::vector<Tensor> norm_backward(const Tensor& dy_, const Tensor& x_,
                  dx.defined() ? dx.mutable_data_ptr() : nullptr,
                  const_cast<float*>(floats(dw)),
                  const_cast<float*>(floats(db)), space.mutable_data_ptr(),
-                 need, word(status), stream_of(x)),
+                 need, stream_of(x)),
          "group_norm_grad");
     return {dx, dw, db};
 }
@@ -207,18 +199,17 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
                           const Tensor& x_, int64_t groups,
                           const optional<Tensor>& weight_,
                           const optional<Tensor>& bias_, double eps,
-                          int64_t activation, const optional<Tensor>& status) {
+                          int64_t activation) {
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor x = x_.contiguous();
         const Tensor weight = weight_.value_or(Tensor());
         const Tensor bias = bias_.value_or(Tensor());
         auto out = norm_forward(x, groups, weight, bias, eps, int(activation),
-                                true, status);
+                                true);
         ctx->save_for_backward({x, weight, bias, out[1], out[2]});
         ctx->saved_data["groups"] = groups;
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["activation"] = activation;
-        ctx->saved_data["status"] = status;
         return out[0];
     }
 
@@ -238,8 +229,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
                               ctx->needs_input_grad(0),
                               s[1].defined() && ctx->needs_input_grad(1),
                               s[2].defined() &&
-                                      ctx->needs_input_grad(at_bias),
-                              ctx->saved_data["status"].toOptional<Tensor>());
+                                      ctx->needs_input_grad(at_bias));
         }
         if (at::GradMode::is_enabled()) {
             // a second derivative is an error, not a silent zero
@@ -250,15 +240,13 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
             for (const Tensor& t : g)
                 if (t.defined()) torch::autograd::set_history(t, error);
         }
-        return {g[0],     Tensor(), g[1],    g[2],
-                Tensor(), Tensor(), Tensor()};
+        return {g[0], Tensor(), g[1], g[2], Tensor(), Tensor()};
     }
 };
 
 Tensor group_norm(const Tensor& x, int64_t groups,
                   optional<Tensor> weight, optional<Tensor> bias, double eps,
-                  const std::string& activation,
-                  const optional<Tensor>& status) {
+                  const std::string& activation) {
     const int act = activation_of(activation);
     bool grad = x.requires_grad();
     for (optional<Tensor>* t : {&weight, &bias})
@@ -268,10 +256,9 @@ Tensor group_norm(const Tensor& x, int64_t groups,
             grad |= (*t)->requires_grad();
         }
     if (grad && at::GradMode::is_enabled())
-        return GroupNorm::apply(x, groups, weight, bias, eps, int64_t(act),
-                                status);
+        return GroupNorm::apply(x, groups, weight, bias, eps, int64_t(act));
     return norm_forward(x, groups, weight.value_or(Tensor()),
-                        bias.value_or(Tensor()), eps, act, false, status)[0];
+                        bias.value_or(Tensor()), eps, act, false)[0];
 }
 
 // --------------------------------------------------------------------- norm
@@ -512,22 +499,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("group_norm_forward",
           [](const Tensor& x, int64_t groups, const optional<Tensor>& w,
              const optional<Tensor>& b, double eps, const std::string& act,
-             bool stats, const optional<Tensor>& status) {
+             bool stats) {
               at::NoGradGuard none;
               return norm_forward(x, groups, w.value_or(Tensor()),
                                   b.value_or(Tensor()), eps,
-                                  activation_of(act), stats, status);
+                                  activation_of(act), stats);
           });
     m.def("group_norm_backward",
           [](const Tensor& dy, const Tensor& x, int64_t groups,
              const optional<Tensor>& w, const optional<Tensor>& b,
              const Tensor& mean, const Tensor& rstd, double eps,
-             const std::string& act, bool wx, bool ww, bool wb,
-             const optional<Tensor>& status) {
+             const std::string& act, bool wx, bool ww, bool wb) {
               at::NoGradGuard none;
               return norm_backward(dy, x, groups, w.value_or(Tensor()),
                                    b.value_or(Tensor()), mean, rstd, eps,
-                                   activation_of(act), wx, ww, wb, status);
+                                   activation_of(act), wx, ww, wb);
           });
     m.def("grad_norm", &grad_norm);
     m.def("dense", &dense);

@@ -101,7 +101,7 @@ def _new_status(device):
 def check_status(device=None, reset: bool = True) -> int:
     """Synchronises with `device` (a device, a tensor on it, or None for
     the current device) and raises DressiError if a kernel reported an
-    error since the last check; reset clears the word."""
+    index error since the last check; reset clears the word."""
     if isinstance(device, torch.Tensor):
         device = device.device
     w = status_word(device)
@@ -111,9 +111,6 @@ def check_status(device=None, reset: bool = True) -> int:
     if word & N.STATUS_INDEX_RANGE:
         raise N.DressiError(N.ERR_DEVICE,
                             "index out of range (face or vertex id)")
-    if word & N.STATUS_WAIT_LIMIT:
-        raise N.DressiError(N.ERR_DEVICE, "thread blocks of a kernel lost one "
-                            "another: its results are incomplete")
     return word
 
 
@@ -728,7 +725,7 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
     "relu" or "silu". With `stats` also the mean and 1 / deviation
     [N, num_groups] that group_norm_grad takes."""
     y, mean, rstd = binding().group_norm_forward(
-        x, num_groups, weight, bias, eps, activation, stats, _word_of(x))
+        x, num_groups, weight, bias, eps, activation, stats)
     return (y, mean, rstd) if stats else y
 
 
@@ -738,19 +735,7 @@ def group_norm_grad(dy, x, num_groups: int, weight, bias, mean, rstd,
     """(dx, dweight, dbias) of group_norm for dy, from x and its statistics;
     None where `want` says so or where weight / bias is None."""
     return tuple(binding().group_norm_backward(
-        dy, x, num_groups, weight, bias, mean, rstd, eps, activation, *want,
-        _word_of(x)))
-
-
-def _word_of(t):
-    """The status word of a tensor's device, or None (not a CUDA tensor; a
-    first use within a capture, whose memory is the graph's)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        return None
-    w = _words.get(t.device.index)
-    if w is None and not torch.cuda.is_current_stream_capturing():
-        w = status_word(t.device)
-    return w
+        dy, x, num_groups, weight, bias, mean, rstd, eps, activation, *want))
 
 
 def grad_norm(tensors, out=None) -> torch.Tensor:

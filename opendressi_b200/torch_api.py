@@ -728,4 +728,4 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
                               activation)[0]
     # outside of a trace the same calls with their autograd in C++
     return ops.binding().group_norm(x, num_groups, weight, bias, eps,
-                                    activation, ops._word_of(x))
+                                    activation)

@@ -42,9 +42,9 @@ def test_group_norm_descriptor(kw, text):
     refused("dressi_group_norm_workspace", C.byref(d), 0, C.byref(size),
             text=text)
     refused("dressi_group_norm", C.byref(d), FAKE, None, None, FAKE, None,
-            None, FAKE, 1 << 40, None, None, text=text)
+            None, FAKE, 1 << 40, None, text=text)
     refused("dressi_group_norm_grad", C.byref(d), FAKE, FAKE, None, None,
-            FAKE, FAKE, FAKE, None, None, FAKE, 1 << 40, None, None, text=text)
+            FAKE, FAKE, FAKE, None, None, FAKE, 1 << 40, None, text=text)
 
 
 def test_group_norm_pointers_and_workspace():
@@ -55,26 +55,26 @@ def test_group_norm_pointers_and_workspace():
     assert need > 0
     big = 1 << 30
     refused("dressi_group_norm", None, FAKE, None, None, FAKE, None, None,
-            FAKE, big, None, None, text="null pointer")
+            FAKE, big, None, text="null pointer")
     refused("dressi_group_norm", C.byref(d), None, None, None, FAKE, None,
-            None, FAKE, big, None, None, text="null pointer")
+            None, FAKE, big, None, text="null pointer")
     refused("dressi_group_norm", C.byref(d), FAKE, None, None, FAKE, FAKE,
-            None, FAKE, big, None, None, text="mean and rstd")
+            None, FAKE, big, None, text="mean and rstd")
     refused("dressi_group_norm", C.byref(d), C.c_void_p((1 << 20) + 2), None,
-            None, FAKE, None, None, FAKE, big, None, None, text="aligned")
+            None, FAKE, None, None, FAKE, big, None, text="aligned")
     refused("dressi_group_norm", C.byref(d), FAKE, None, None, FAKE, None,
-            None, FAKE, need - 1, None, None, text="too small")
+            None, FAKE, need - 1, None, text="too small")
     refused("dressi_group_norm", C.byref(d), FAKE, None, None, FAKE, None,
-            None, C.c_void_p((1 << 20) + 8), big, None, None, text="16 bytes")
+            None, C.c_void_p((1 << 20) + 8), big, None, text="16 bytes")
     refused("dressi_group_norm_grad", C.byref(d), FAKE, FAKE, None, None,
-            None, FAKE, FAKE, None, None, FAKE, big, None, None,
+            None, FAKE, FAKE, None, None, FAKE, big, None,
             text="null pointer")
     refused("dressi_group_norm_workspace", C.byref(d), 0, None,
             text="null pointer")
     # nothing to do: accepted with null images
     empty = norm_desc(n=0)
     assert N.load().dressi_group_norm(C.byref(empty), None, None, None, None,
-                                      None, None, None, 0, None, None) == N.OK
+                                      None, None, None, 0, None) == N.OK
 
 
 def test_grad_norm_arguments():
