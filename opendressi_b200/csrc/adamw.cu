@@ -27,6 +27,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -67,7 +68,8 @@ struct AdamWHyper {
     uint32_t* ticket;
 };
 
-// The tensors of a launch; 400 fill the 32764 bytes of a kernel's arguments.
+// The tensors of a launch; 400 fill the 32764 bytes of a kernel's arguments
+// (which then take 3 us longer to launch: three sizes).
 template <int CAP>
 struct AdamWTable {
     void* p[CAP];
@@ -595,6 +597,7 @@ template <typename T, int BITS, int CAP>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<BITS>())
         k_adamw(const __grid_constant__ AdamWTable<CAP> t,
                 const __grid_constant__ AdamWHyper h) {
+    await_previous();  // the norm, where this launch began early
     using State = typename StateOf<BITS>::type;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint64_t all = t.first[t.count];
@@ -668,7 +671,7 @@ bool aligned(const void* p, size_t a) {
 
 template <typename T, int BITS, int CAP>
 void launch_adamw(const AdamWArgs& a, const AdamWHyper& h, uint32_t i0,
-                  uint32_t i1, cudaStream_t s) {
+                  uint32_t i1, bool early, cudaStream_t s) {
     AdamWTable<CAP> t;
     t.count = i1 - i0;
     uint64_t blocks = 0;
@@ -708,14 +711,21 @@ void launch_adamw(const AdamWArgs& a, const AdamWHyper& h, uint32_t i0,
         DRESSI_CUDA(cudaFuncSetAttribute(
                 k_adamw<T, BITS, CAP>,
                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    k_adamw<T, BITS, CAP><<<unsigned(grid), kThreads, smem, s>>>(t, h);
-    DRESSI_CUDA(cudaGetLastError());
+    if (early) {
+        launch_early(k_adamw<T, BITS, CAP>, dim3(unsigned(grid)), kThreads,
+                     smem, s, t, h);
+    } else {
+        k_adamw<T, BITS, CAP><<<unsigned(grid), kThreads, smem, s>>>(t, h);
+        DRESSI_CUDA(cudaGetLastError());
+    }
 }
 
 template <typename T, int BITS>
 void adamw_t(const AdamWArgs& a, const AdamWHyper& h, cudaStream_t s) {
-    constexpr uint32_t kFew = 32, kMany = 400;
+    constexpr uint32_t kFew = 32, kSome = 128, kMany = 400;
     for (uint32_t i0 = 0; i0 < a.n_tensors;) {
+        // behind the norm's launch, which lets it
+        const bool early = h.norm && i0 == 0;
         uint32_t i1 = i0;
         uint64_t blocks = 0;
         while (i1 < a.n_tensors && i1 - i0 < kMany) {
@@ -724,45 +734,71 @@ void adamw_t(const AdamWArgs& a, const AdamWHyper& h, cudaStream_t s) {
             blocks += more;
             i1++;
         }
-        if (i1 - i0 <= kFew) launch_adamw<T, BITS, kFew>(a, h, i0, i1, s);
-        else launch_adamw<T, BITS, kMany>(a, h, i0, i1, s);
+        if (i1 - i0 <= kFew) launch_adamw<T, BITS, kFew>(a, h, i0, i1, early, s);
+        else if (i1 - i0 <= kSome)
+            launch_adamw<T, BITS, kSome>(a, h, i0, i1, early, s);
+        else launch_adamw<T, BITS, kMany>(a, h, i0, i1, early, s);
         i0 = i1;
     }
 }
 
 // --------------------------------------------------------------------- norm
 
-constexpr int kNormCap = 1000;
 constexpr int kNormUnit = kThreads * kLane;  // values a thread block takes
 constexpr int kNormCtasPerSm = 4;
-constexpr int kNormMost = 1024;              // thread blocks (partial sums)
+// Thread blocks (partial sums): more than fit, so that one with many small
+// tensors, each a wait for memory, keeps none waiting.
+constexpr int kNormMost = 2368;
 
+// A launch takes longer the more arguments it has (2.8 us with 4 kB, 4.9 with
+// 21 kB), so tables come in three sizes.
+template <int CAP>
 struct NormTable {
-    const void* p[kNormCap];
-    uint64_t n[kNormCap];
-    uint32_t first[kNormCap + 1];
-    uint8_t type[kNormCap];
+    const void* p[CAP];
+    uint64_t n[CAP];
+    uint32_t first[CAP + 1];
+    uint8_t type[CAP];
     uint32_t count;
 };
 
 // Squares are summed in 64 bits from the first on: no overflow, and an order
-// that depends on the sizes alone.
+// that depends on the sizes and alignments alone. Units q .. stop - 1 of a
+// tensor, four loads under way together.
 template <typename T>
-__device__ __forceinline__ double squares(const T* p, uint64_t left) {
+__device__ __forceinline__ double squares(const T* p, uint64_t n, uint32_t q,
+                                          uint32_t stop) {
     double s = 0.0;
-    float x[kLane];
-    if (left >= kNormUnit &&
-        reinterpret_cast<uintptr_t>(p) % (kLane * sizeof(T)) == 0) {
-        load8(p + threadIdx.x * kLane, x);
-    } else {
+    auto add = [&](const float* x) {
 #pragma unroll
-        for (int j = 0; j < kLane; j++) {
-            const uint32_t at = threadIdx.x + kThreads * j;
-            x[j] = at < left ? to_f(p[at]) : 0.f;
+        for (int j = 0; j < kLane; j++) s += double(x[j]) * double(x[j]);
+    };
+    if (reinterpret_cast<uintptr_t>(p) % (kLane * sizeof(T)) == 0) {
+        const uint32_t whole = uint32_t(min(uint64_t(stop), n / kNormUnit));
+        const T* at = p + uint64_t(q) * kNormUnit + threadIdx.x * kLane;
+        for (; q + 4 <= whole; q += 4, at += 4 * kNormUnit) {
+            float x[4][kLane];
+#pragma unroll
+            for (int k = 0; k < 4; k++) load8(at + k * kNormUnit, x[k]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) add(x[k]);
+        }
+        for (; q < whole; q++, at += kNormUnit) {
+            float x[kLane];
+            load8(at, x);
+            add(x);
         }
     }
+    for (; q < stop; q++) {
+        const T* at = p + uint64_t(q) * kNormUnit;
+        const uint64_t left = n - uint64_t(q) * kNormUnit;
+        float x[kLane];
 #pragma unroll
-    for (int j = 0; j < kLane; j++) s += double(x[j]) * double(x[j]);
+        for (int j = 0; j < kLane; j++) {
+            const uint32_t i = threadIdx.x + kThreads * j;
+            x[j] = i < left ? to_f(at[i]) : 0.f;
+        }
+        add(x);
+    }
     return s;
 }
 
@@ -777,25 +813,31 @@ __device__ __forceinline__ double block_sum(double s) {
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads)
-        k_norm_parts(const __grid_constant__ NormTable t, double* part,
+template <int CAP>
+__global__ void __launch_bounds__(kThreads, kNormCtasPerSm)
+        k_norm_parts(const __grid_constant__ NormTable<CAP> t, double* part,
                      int add) {
+    start_next();
     const uint64_t all = t.first[t.count];
     const uint32_t end = uint32_t(all * (blockIdx.x + 1) / gridDim.x);
+    uint32_t b = uint32_t(all * blockIdx.x / gridDim.x);
     double s = 0.0;
-    uint32_t ti = kNone;
-    for (uint32_t b = uint32_t(all * blockIdx.x / gridDim.x); b < end; b++) {
-        if (ti == kNone) ti = tensor_of(t, b);
+    uint32_t ti = b < end ? tensor_of(t, b) : 0u;
+    while (b < end) {
         while (b >= t.first[ti + 1]) ti++;
-        const uint64_t at = uint64_t(b - t.first[ti]) * kNormUnit;
-        const uint64_t left = t.n[ti] - at;
+        const uint32_t first = t.first[ti];
+        const uint32_t stop = min(end, t.first[ti + 1]);
+        const uint64_t n = t.n[ti];
         if (t.type[ti] == 0)
-            s += squares(static_cast<const float*>(t.p[ti]) + at, left);
+            s += squares(static_cast<const float*>(t.p[ti]), n, b - first,
+                         stop - first);
         else if (t.type[ti] == 1)
-            s += squares(static_cast<const __half*>(t.p[ti]) + at, left);
+            s += squares(static_cast<const __half*>(t.p[ti]), n, b - first,
+                         stop - first);
         else
-            s += squares(static_cast<const __nv_bfloat16*>(t.p[ti]) + at,
-                         left);
+            s += squares(static_cast<const __nv_bfloat16*>(t.p[ti]), n,
+                         b - first, stop - first);
+        b = stop;
     }
     s = block_sum(s);
     if (threadIdx.x == 0)
@@ -804,6 +846,8 @@ __global__ void __launch_bounds__(kThreads)
 
 __global__ void __launch_bounds__(kThreads)
         k_norm_finish(const double* part, int n, float* out) {
+    start_next();
+    await_previous();
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += kThreads) s += part[i];
     s = block_sum(s);
@@ -858,15 +902,16 @@ void grad_norm_op(uint32_t n_tensors, const void* const* tensors,
     for (uint32_t i = 0; i < n_tensors; i++) all += units(i);
     const int grid = int(std::max<uint64_t>(
             1, std::min<uint64_t>(
-                       all, std::min(kNormMost, sm_count() * kNormCtasPerSm))));
+                       all, std::min(kNormMost, sm_count() * 16))));
     ProfScope ps("grad_norm", s);
     uint32_t i = 0;
     int add = 0;
-    do {
-        NormTable t;
+    auto run = [&](auto cap) {
+        constexpr uint32_t kCap = decltype(cap)::value;
+        NormTable<kCap> t;
         uint64_t blocks = 0;
         uint32_t k = 0;
-        for (; i < n_tensors && k < kNormCap; i++, k++) {
+        for (; i < n_tensors && k < kCap; i++, k++) {
             if (k > 0 && blocks + units(i) > kMostBlocks) break;
             t.p[k] = tensors[i];
             t.n[k] = numel[i];
@@ -876,12 +921,18 @@ void grad_norm_op(uint32_t n_tensors, const void* const* tensors,
         }
         t.first[k] = uint32_t(blocks);
         t.count = k;
-        k_norm_parts<<<grid, kThreads, 0, s>>>(t, part, add);
+        k_norm_parts<kCap><<<grid, kThreads, 0, s>>>(t, part, add);
         DRESSI_CUDA(cudaGetLastError());
         add = 1;
+    };
+    do {
+        const uint32_t left = n_tensors - i;
+        if (left <= 32) run(std::integral_constant<uint32_t, 32>());
+        else if (left <= 192) run(std::integral_constant<uint32_t, 192>());
+        else run(std::integral_constant<uint32_t, 1000>());
     } while (i < n_tensors);
-    k_norm_finish<<<1, kThreads, 0, s>>>(part, grid, out);
-    DRESSI_CUDA(cudaGetLastError());
+    launch_early(k_norm_finish, dim3(1), kThreads, 0, s,
+                 static_cast<const double*>(part), grid, out);
 }
 
 }  // namespace dressi

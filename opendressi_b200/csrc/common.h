@@ -103,6 +103,34 @@ struct ProfScope {
     }
 };
 
+// Launches a kernel that may begin while the one before it in the stream still
+// runs: it calls await_previous() before it touches what that one (or an
+// earlier one) reads or writes. The one before calls start_next() where its
+// own work may overlap with such a beginning.
+template <typename... P, typename... A>
+void launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                  cudaStream_t s, A... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3(unsigned(threads));
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &early;
+    c.numAttrs = 1;
+    DRESSI_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ void await_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void start_next() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+#endif
+
 // Bump allocator over one device block (plans and op-level workspaces).
 struct Arena {
     char* base = nullptr;

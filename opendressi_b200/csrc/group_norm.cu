@@ -275,13 +275,13 @@ __device__ __forceinline__ void copy_16(void* to, const void* from) {
                  : "memory");
 }
 
-// Calls fn(a, b) for `steps` vectors of one image (q null) or two. Whole
-// vectors come through a ring in shared memory, each thread's its own: loads
+// Calls ready() once the first loads are under way, then fn(a, b) for `steps`
+// vectors of one image (q null) or two. Whole vectors come through a ring in shared memory, each thread's its own: loads
 // into registers would be a quarter as many.
-template <typename T, int VEC, int IMAGES, typename F>
+template <typename T, int VEC, int IMAGES, typename R, typename F>
 __device__ __forceinline__ void walk_over(const T* p, const T* q,
                                           uint64_t step, uint32_t steps,
-                                          char* ring, F&& fn) {
+                                          char* ring, R&& ready, F&& fn) {
     using V = Pack<T, VEC>;
     if constexpr (whole_vectors<T, VEC>()) {
         constexpr int stage = 2 * IMAGES * kGnThreads;
@@ -306,6 +306,7 @@ __device__ __forceinline__ void walk_over(const T* p, const T* q,
         };
 #pragma unroll
         for (int k = 0; k < kGnStages; k++) send(own + k * stage);
+        ready();
         V* slot = own;
         for (uint32_t t = 0; t < steps; t += 2) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kGnStages - 1)
@@ -326,6 +327,7 @@ __device__ __forceinline__ void walk_over(const T* p, const T* q,
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         constexpr int kBatch = 4 / IMAGES;  // loads under way together
+        ready();
         uint32_t t = 0;
         for (; t + kBatch <= steps; t += kBatch) {
             V a[kBatch], b[kBatch];
@@ -526,13 +528,14 @@ __global__ void __launch_bounds__(kGnThreads)
     const uint32_t chunk =
             d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
     const uint64_t n = blockIdx.y;
+    start_next();
     const Walk w = walk_of<VEC>(d, chunk, slab);
     ThreadMoments<VEC> m;
     if (w.steps > 0) {
         const T* own = x + n * d.rows * d.C + w.base;
-        m.begin(load_pack<T, VEC>(own));
         walk_over<T, VEC, 1>(
                 own, static_cast<const T*>(nullptr), w.step, w.steps, ring,
+                [&] { m.begin(load_pack<T, VEC>(own)); },
                 [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) { m.add(v); });
     }
     // the ring is free once every thread has left it
@@ -563,10 +566,12 @@ __device__ __forceinline__ double part_count(const GnDims& d, uint32_t e) {
 
 // mean[n][g], rstd[n][g] from the parts; one warp each.
 __global__ void k_gn_finish(GnDims d, uint32_t n,
-                            const double2* __restrict__ part,
+                            const double2* part,
                             float* __restrict__ mean,
                             float* __restrict__ rstd) {
     const uint64_t i = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
+    start_next();
+    await_previous();
     if (i >= uint64_t(n) * d.G) return;
     const uint32_t np = d.chunks * d.pieces;
     const double2* own = part + i * np;
@@ -591,8 +596,8 @@ __global__ void __launch_bounds__(kGnThreads)
         k_gn_apply(GnDims d, const T* __restrict__ x,
                    const float* __restrict__ weight,
                    const float* __restrict__ bias,
-                   const float* __restrict__ mean,
-                   const float* __restrict__ rstd, T* __restrict__ y) {
+                   const float* mean,
+                   const float* rstd, T* __restrict__ y) {
     extern __shared__ __align__(16) char ring[];
     // the last chunks first: they are what the statistics pass left on chip
     const uint32_t i = gridDim.x - 1 - blockIdx.x;
@@ -603,7 +608,8 @@ __global__ void __launch_bounds__(kGnThreads)
     if (w.steps == 0) return;
     constexpr int P = kPairs<VEC>;
     Two mu[P], a[P], b[P];
-    {
+    auto scales = [&] {
+        await_previous();
         float m1[2 * P], a1[2 * P], b1[2 * P];
         each_channel<VEC>(d, w, [&](int j, int c, int g) {
             m1[j] = -mean[n * d.G + g];
@@ -617,11 +623,11 @@ __global__ void __launch_bounds__(kGnThreads)
             a[j] = two(a1[2 * j], a1[2 * j + 1]);
             b[j] = two(b1[2 * j], b1[2 * j + 1]);
         }
-    }
+    };
     T* to = y + n * d.rows * d.C + w.base;
     walk_over<T, VEC, 1>(
             x + n * d.rows * d.C + w.base, static_cast<const T*>(nullptr),
-            w.step, w.steps, ring,
+            w.step, w.steps, ring, scales,
             [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) {
                 Two e[P];
                 unpack<T, VEC>(v, e);
@@ -821,17 +827,20 @@ __global__ void __launch_bounds__(kGnThreads)
     const uint32_t chunk =
             d.slabs == 1 ? blockIdx.x : blockIdx.x / uint32_t(d.slabs);
     const uint64_t n = blockIdx.y;
+    start_next();
     const Walk w = walk_of<VEC>(d, chunk, slab);
     constexpr int P = kPairs<VEC>;
     Two A[P], B[P];
     if (w.works) {
-        const Scales<VEC> c =
-                scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
+        Scales<VEC> c;
 #pragma unroll
         for (int j = 0; j < P; j++) A[j] = B[j] = two(0.f);
         const uint64_t at = n * d.rows * d.C + w.base;
         walk_over<T, VEC, 2>(
                 x + at, dy + at, w.step, w.steps, ring,
+                [&] {
+                    c = scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
+                },
                 [&](const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
                     Two h[P], g[P];
                     unpack<T, VEC>(v, h);
@@ -878,6 +887,8 @@ __global__ void __launch_bounds__(512)
     __shared__ double sa[16][33], sb[16][33];
     const int bundles = (d.G + bundle - 1) / bundle;
     const uint64_t n = blockIdx.x / bundles;
+    start_next();
+    await_previous();
     const int g0 = int(blockIdx.x % bundles) * bundle;
     const int groups = min(bundle, d.G - g0);
     const int lane = threadIdx.x & 31, row = threadIdx.x / 32;
@@ -932,7 +943,7 @@ __global__ void __launch_bounds__(kGnThreads)
                         const float* __restrict__ bias,
                         const float* __restrict__ mean,
                         const float* __restrict__ rstd,
-                        const float2* __restrict__ means,
+                        const float2* means,
                         T* __restrict__ dx) {
     extern __shared__ __align__(16) char ring[];
     const uint32_t i = gridDim.x - 1 - blockIdx.x;
@@ -942,9 +953,11 @@ __global__ void __launch_bounds__(kGnThreads)
     const Walk w = walk_of<VEC>(d, chunk, slab);
     if (w.steps == 0) return;
     constexpr int P = kPairs<VEC>;
-    const Scales<VEC> c = scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
+    Scales<VEC> c;
     Two ma[P], mb[P];
-    {
+    auto scales = [&] {
+        c = scales_of<VEC>(d, w, n, weight, bias, mean, rstd);
+        await_previous();
         float a1[2 * P], b1[2 * P];
         each_channel<VEC>(d, w, [&](int j, int, int g) {
             const float2 m = means[n * d.G + g];
@@ -957,11 +970,11 @@ __global__ void __launch_bounds__(kGnThreads)
             ma[j] = two(a1[2 * j], a1[2 * j + 1]);
             mb[j] = two(b1[2 * j], b1[2 * j + 1]);
         }
-    }
+    };
     const uint64_t at = n * d.rows * d.C + w.base;
     T* to = dx + at;
     walk_over<T, VEC, 2>(
-            x + at, dy + at, w.step, w.steps, ring,
+            x + at, dy + at, w.step, w.steps, ring, scales,
             [&](const Pack<T, VEC>& v, const Pack<T, VEC>& e) {
                 Two h[P], g[P];
                 unpack<T, VEC>(v, h);
@@ -1121,12 +1134,13 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
 // dweight[c], dbias[c] = the sums over `rows` rows of sums[row][c], in an
 // order that their number gives: 32 columns x 16 lanes a block.
 __global__ void __launch_bounds__(512)
-        k_gn_grad_affine(int C, uint64_t rows, const float2* __restrict__ sums,
+        k_gn_grad_affine(int C, uint64_t rows, const float2* sums,
                          float* __restrict__ dweight,
                          float* __restrict__ dbias) {
     __shared__ double sa[16][33], sb[16][33];
     const int lane = threadIdx.x & 31, row = threadIdx.x / 32;
     const int c = blockIdx.x * 32 + lane;
+    await_previous();
     double a = 0.0, b = 0.0;
     if (c < C) {
 #pragma unroll 8
@@ -1306,12 +1320,17 @@ GnWorkspace carve(const GroupNormArgs& a, const GnPlan& p, bool grad,
     return w;
 }
 
-// Launches a kernel with a ring of `smem` bytes.
+// Launches a kernel with `smem` bytes of dynamic shared memory; early: it may
+// begin while the launch before still runs (which is one of this file).
 template <typename... P, typename... A>
-void launch(void (*kernel)(P...), dim3 grid, int smem, cudaStream_t s,
-            A... args) {
+void launch(void (*kernel)(P...), dim3 grid, int smem, bool early,
+            cudaStream_t s, A... args) {
     DRESSI_CUDA(cudaFuncSetAttribute(
             kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (early) {
+        launch_early(kernel, grid, kGnThreads, size_t(smem), s, args...);
+        return;
+    }
     kernel<<<grid, kGnThreads, smem, s>>>(args...);
     DRESSI_CUDA(cudaGetLastError());
 }
@@ -1324,7 +1343,7 @@ void forward_t(const GnPlan& p, const GroupNormArgs& a, const void* x,
         launch(a.act == 1   ? k_gn_resident<T, VEC, 1>
                : a.act == 2 ? k_gn_resident<T, VEC, 2>
                             : k_gn_resident<T, VEC, 0>,
-               dim3(p.grid), p.smem, s, p.d, p.items,
+               dim3(p.grid), p.smem, false, s, p.d, p.items,
                static_cast<const T*>(x), weight, bias, mean, rstd,
                static_cast<T*>(y));
         return;
@@ -1342,13 +1361,14 @@ void forward_t(const GnPlan& p, const GroupNormArgs& a, const void* x,
         float* mb = mean + n0 * a.G;
         float* rb = rstd + n0 * a.G;
         constexpr int smem = ring_bytes<T, VEC>(1);
-        launch(k_gn_stats<T, VEC>, grid, smem, s, p.d, xb, w.part);
-        k_gn_finish<<<unsigned((nb * a.G + 7) / 8), 256, 0, s>>>(
-                p.d, uint32_t(nb), w.part, mb, rb);
+        launch(k_gn_stats<T, VEC>, grid, smem, false, s, p.d, xb, w.part);
+        launch_early(k_gn_finish, dim3(unsigned((nb * a.G + 7) / 8)), 256, 0,
+                     s, p.d, uint32_t(nb), static_cast<const double2*>(w.part),
+                     mb, rb);
         launch(a.act == 1   ? k_gn_apply<T, VEC, 1>
                : a.act == 2 ? k_gn_apply<T, VEC, 2>
                             : k_gn_apply<T, VEC, 0>,
-               grid, smem, s, p.d, xb, weight, bias,
+               grid, smem, true, s, p.d, xb, weight, bias,
                static_cast<const float*>(mb), static_cast<const float*>(rb),
                yb);
     }
@@ -1362,13 +1382,13 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
                 cudaStream_t s) {
     auto affine = [&](uint64_t rows) {
         if (!dweight && !dbias) return;
-        k_gn_grad_affine<<<unsigned((a.C + 31) / 32), 512, 0, s>>>(
-                a.C, rows, w.sums, dweight, dbias);
-        DRESSI_CUDA(cudaGetLastError());
+        launch_early(k_gn_grad_affine, dim3(unsigned((a.C + 31) / 32)), 512, 0,
+                     s, a.C, rows, static_cast<const float2*>(w.sums), dweight,
+                     dbias);
     };
     if (p.items) {
-        launch(k_gn_resident_grad<T, VEC, ACT>, dim3(p.grid), p.smem, s, p.d,
-               p.items, static_cast<const T*>(dy), static_cast<const T*>(x),
+        launch(k_gn_resident_grad<T, VEC, ACT>, dim3(p.grid), p.smem, false, s,
+               p.d, p.items, static_cast<const T*>(dy), static_cast<const T*>(x),
                weight, bias, mean, rstd, w.sums, static_cast<T*>(dx));
         affine(a.n);
         return;
@@ -1385,14 +1405,14 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
         const float* rb = rstd + n0 * a.G;
         float2* means = w.means + n0 * a.G;
         constexpr int smem = ring_bytes<T, VEC>(2);
-        launch(k_gn_grad_sums<T, VEC, ACT>, grid, smem, s, p.d, gb, xb, weight,
-               bias, mb, rb, w.sums_part);
-        k_gn_grad_finish<<<unsigned(nb * bundles), 512, 0, s>>>(
-                p.d, bundle, w.sums_part, weight, w.sums + n0 * a.C, means);
-        DRESSI_CUDA(cudaGetLastError());
+        launch(k_gn_grad_sums<T, VEC, ACT>, grid, smem, false, s, p.d, gb, xb,
+               weight, bias, mb, rb, w.sums_part);
+        launch_early(k_gn_grad_finish, dim3(unsigned(nb * bundles)), 512, 0, s,
+                     p.d, bundle, static_cast<const float2*>(w.sums_part),
+                     weight, w.sums + n0 * a.C, means);
         if (dx)
-            launch(k_gn_grad_apply<T, VEC, ACT>, grid, smem, s, p.d, gb, xb,
-                   weight, bias, mb, rb, static_cast<const float2*>(means),
+            launch(k_gn_grad_apply<T, VEC, ACT>, grid, smem, true, s, p.d, gb,
+                   xb, weight, bias, mb, rb, static_cast<const float2*>(means),
                    static_cast<T*>(dx) + n0 * sample);
     }
     affine(a.n);
