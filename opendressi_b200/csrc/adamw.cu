@@ -6,8 +6,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // with g first scaled by min(1, max_norm / (norm + 1e-6)) when clipping, and p
-// clamped last. Bound by memory: 28 bytes a value with f32 parameters and 32-bit moments,
-// 16 + 8/256 with 8-bit ones.
+// clamped last. Bound by memory: 28 bytes a value with f32 parameters and
+// 32-bit moments, 16 + 16/256 with 8-bit ones.
 //
 // The tensors' addresses travel as a kernel argument (no table to upload, so
 // a step can be captured), the work is cut into blocks of 256 values of one
@@ -23,7 +23,7 @@
 // probability of their place between the two neighbours. The 16 random bits
 // for each come from Wang's hash of (seed, step, tensor, place), so a run
 // repeats exactly. r > 0 is never rounded to 0: m / (0 + eps) would explode.
-// What is not finite is stored as NaN and leaves the block's scale alone.
+// (A root below 2^-63 counts as 0 where eps is 2^-40 or more.) What is not finite is stored as NaN and leaves the block's scale alone.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -54,7 +54,6 @@ template <int BITS>
 constexpr int ctas_per_sm() {
     return BITS == 8 ? kCtasPerSm8 : kCtasPerSm;
 }
-constexpr uint32_t kNone = 0xffffffffu;
 constexpr uint64_t kMostBlocks = 1ull << 31;  // of one launch
 
 struct AdamWHyper {
@@ -287,13 +286,13 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t* b) {
 // and below 2^-6 (there 2^-126) both are equally spaced. 16 random bits and a
 // half are added to those 20 and what carries goes up: up with the probability
 // of the value's place between its neighbours. (All of it is moved up by 4
-// bits, which drops the sign: a code is then the highest byte.) inv is within
-// 3 * 2^-24 of its value: the largest comes out below 448 + 8 * 2^-15 and
-// never carries past 448.
+// bits, which drops the sign: a code is then the highest byte.) inv and the
+// product are rounded: the largest comes out below 448 + 8 * 2^-15 and never
+// carries past 448.
 template <bool ROOT>
 __device__ __forceinline__ uint2 encode(const float* x, float top, bool finite,
                                         const uint32_t* bits) {
-    const float inv = 448.f * rcp_fast(top);
+    const float inv = 448.f / top;
     uint32_t b[kLane];
     float z[kLane];
     // one product where inv 2^-120 is no denormal number
@@ -745,10 +744,8 @@ void adamw_t(const AdamWArgs& a, const AdamWHyper& h, cudaStream_t s) {
 // --------------------------------------------------------------------- norm
 
 constexpr int kNormUnit = kThreads * kLane;  // values a thread block takes
-constexpr int kNormCtasPerSm = 4;
-// Thread blocks (partial sums): more than fit, so that one with many small
-// tensors, each a wait for memory, keeps none waiting.
-constexpr int kNormMost = 2368;
+constexpr int kNormCtasPerSm = 4;  // one wave: more blocks were slower
+constexpr int kNormMost = 1024;    // thread blocks (partial sums)
 
 // A launch takes longer the more arguments it has (2.8 us with 4 kB, 4.9 with
 // 21 kB), so tables come in three sizes.
@@ -849,6 +846,7 @@ __global__ void __launch_bounds__(kThreads)
     start_next();
     await_previous();
     double s = 0.0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += kThreads) s += part[i];
     s = block_sum(s);
     if (threadIdx.x == 0) out[0] = float(sqrt(s));
@@ -902,7 +900,7 @@ void grad_norm_op(uint32_t n_tensors, const void* const* tensors,
     for (uint32_t i = 0; i < n_tensors; i++) all += units(i);
     const int grid = int(std::max<uint64_t>(
             1, std::min<uint64_t>(
-                       all, std::min(kNormMost, sm_count() * 16))));
+                       all, std::min(kNormMost, sm_count() * kNormCtasPerSm))));
     ProfScope ps("grad_norm", s);
     uint32_t i = 0;
     int add = 0;
