@@ -1221,17 +1221,24 @@ int dressi_adamw_step(const dressi_adamw_desc* d, void* stream) {
         const size_t es = dtype_bytes(d->dtype);
         for (uint32_t i = 0; i < d->n_tensors; i++) {
             DRESSI_REQUIRE(d->numel[i] < (1ull << 39), "adamw: too long");
-            DRESSI_REQUIRE(d->steps[i], "adamw: null step counter");
+            DRESSI_REQUIRE(d->steps[i] && aligned_to(d->steps[i], 4),
+                           "adamw: null step counter, or one not aligned");
             if (d->numel[i] == 0) continue;
             DRESSI_REQUIRE(d->params[i] && d->grads[i] && d->exp_avg[i] &&
                                    d->exp_avg_sq[i] &&
                                    (!bits8 || (d->exp_avg_scale[i] &&
                                                d->exp_avg_sq_scale[i])),
                            "adamw: null tensor");
+            const void* first = bits8 ? static_cast<const void*>(
+                                                d->exp_avg_scale[i])
+                                      : d->exp_avg[i];
+            const void* second = bits8 ? static_cast<const void*>(
+                                                 d->exp_avg_sq_scale[i])
+                                       : d->exp_avg_sq[i];
             DRESSI_REQUIRE(aligned_to(d->params[i], es) &&
                                    aligned_to(d->grads[i], es) &&
-                                   (bits8 || (aligned_to(d->exp_avg[i], 4) &&
-                                              aligned_to(d->exp_avg_sq[i], 4))),
+                                   aligned_to(first, 4) &&
+                                   aligned_to(second, 4),
                            "adamw: tensor not aligned to its element");
         }
         AdamWArgs a{};

@@ -1175,7 +1175,8 @@ struct GnPlan {
 };
 
 // A round of launches covers as many samples as stay in L2 between its two
-// passes.
+// passes (67 MB in one round take 45 us, in two 58, in four 90: a round's
+// launches cost 3 us, and what they do not read again is little).
 constexpr uint64_t kGnRoundBytes = 64ull << 20;
 
 bool aligned(const void* p, size_t a) {
@@ -1278,8 +1279,10 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
 
     // Rounds of launches: one wave of blocks, 4 steps or more a thread.
     const uint64_t bytes = std::max<uint64_t>(1, sample * es * images);
-    p.batch = std::min<uint64_t>(std::max<uint64_t>(1, kGnRoundBytes / bytes),
-                                 std::min<uint64_t>(a.n, 65535));
+    const uint64_t rounds = std::max<uint64_t>(
+            (a.n + 65534) / 65535,
+            (a.n - 1) / std::max<uint64_t>(1, kGnRoundBytes / bytes) + 1);
+    p.batch = (a.n + rounds - 1) / rounds;
     uint64_t chunks = std::max<uint64_t>(
             1, uint64_t(kGnSms) * (grad ? 2 : 4) /
                        std::max<uint64_t>(1, p.batch * d.slabs));

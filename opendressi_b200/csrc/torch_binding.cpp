@@ -302,9 +302,10 @@ Tensor grad_norm(const std::vector<Tensor>& tensors,
             a.add(held.back(), dtype);
         }
     }
-    const auto dev = tensors.empty()
-                             ? at::Device(at::kCUDA, c10::cuda::current_device())
-                             : tensors[0].device();
+    const at::Device dev =
+            tensors.empty()
+                    ? at::Device(at::kCUDA, c10::cuda::current_device())
+                    : tensors[0].device();
     const c10::cuda::CUDAGuard guard(dev);
     Tensor out;
     if (out_.has_value()) {
@@ -485,8 +486,9 @@ bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    static py::object error =
-            py::module_::import("opendressi_b200._native").attr("DressiError");
+    // never released: it is used until the interpreter is gone
+    static py::object& error = *new py::object(
+            py::module_::import("opendressi_b200._native").attr("DressiError"));
     py::register_exception_translator([](std::exception_ptr p) {
         try {
             if (p) std::rethrow_exception(p);

@@ -3,7 +3,7 @@
 against a plain restatement of their rounding.
 
 Tolerances count roundings of 2^-24 each (U): two products, a sum and the
-rounded betas for a moment; for the update about a dozen operations with the
+rounded betas for a moment (and half a denormal step for each product); for the update about a dozen operations with the
 bias corrections; a parameter in type T is rounded once, eps(T) / 2."""
 
 import math
@@ -42,7 +42,8 @@ def formula(p, g, m, v, t, lr, betas, eps, wd, coef=1.0, clamp=None):
     m1 = b1 * m + (1 - b1) * g
     m_err = 4 * U * ((b1 * m).abs() + ((1 - b1) * g).abs() * (1 + g_err / U))
     v1 = b2 * v + (1 - b2) * g * g
-    v_err = 5 * U * (b2 * v + (1 - b2) * g * g * (1 + 2 * g_err / U))
+    v_err = 5 * U * (b2 * v + (1 - b2) * g * g * (1 + 2 * g_err / U)) \
+        + 2.0 ** -148  # two products that may be denormal
     c1, c2 = 1 - b1 ** t, 1 - b2 ** t
     den = (v1 / c2).sqrt() + eps
     step = lr / c1 * m1 / den
@@ -105,6 +106,51 @@ def test_steps_in_32_bits(cuda, dtype, max_norm):
             near(st["exp_avg"], m1, me)
             near(st["exp_avg_sq"], v1, ve)
             near(p.detach(), p1, pe)
+
+
+def test_denormal_second_moments(cuda):
+    """With eps 0 the root of a denormal number counts."""
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    p = make(21, [(1000,)], torch.float32)[0]
+    p0 = p.detach().clone()
+    p.grad = 3e-19 * (1 + torch.rand(1000, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-2, betas=(0.9, 0.99), eps=0.0,
+                      weight_decay=0.0)
+    opt.step()
+    z = torch.zeros(1000, device="cuda").double()
+    p1, pe, m1, me, v1, ve = formula(p0, p.grad, z, z, 1, 1e-2, (0.9, 0.99),
+                                     0.0, 0.0)
+    assert float(v1.max()) < 2.0 ** -126
+    near(opt.state[p]["exp_avg_sq"], v1, ve)
+    near(p.detach(), p1, pe)
+
+
+def test_clip_over_groups_and_types(cuda):
+    """One norm for all groups and element types, and a launch for each."""
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    a = make(22, [(700,), (3, 9)], torch.float32, scale=1.0)
+    b = make(23, [(64, 65)], torch.bfloat16, scale=1.0)
+    c = make(24, [(501,)], torch.float16, scale=1.0)
+    params = a + b + c
+    opt = optim.AdamW([{"params": a + b}, {"params": c, "lr": 1e-2}],
+                      lr=1e-3, max_norm=0.25)
+    before = [p.detach().clone() for p in params]
+    norm = math.sqrt(sum(float((p.grad.double() ** 2).sum()) for p in params))
+    opt.step()
+    assert abs(float(opt.last_norm) / norm - 1) <= 2 * U
+    for p, p0 in zip(params, before):
+        z = torch.zeros_like(p0).double()
+        lr = 1e-2 if p is c[0] else 1e-3
+        p1, pe, m1, me, v1, ve = formula(p0, p.grad, z, z, 1, lr,
+                                         (0.9, 0.999), 1e-8, 1e-2,
+                                         0.25 / (norm + 1e-6))
+        near(opt.state[p]["exp_avg"], m1, me)
+        near(opt.state[p]["exp_avg_sq"], v1, ve)
+        near(p.detach(), p1, pe)
 
 
 @pytest.mark.parametrize("bits", [32, 8])

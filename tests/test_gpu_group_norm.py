@@ -124,6 +124,8 @@ SHAPES = [
     ((2, 3, 3, 4096), 32), ((1, 5, 3, 4100), 1), ((2, 2, 3, 5002), 2),
     ((1, 4, 2, 9000), 2), ((2, 3, 1030), 515), ((1, 2, 2, 1021), 1021),
     ((1, 3, 1, 8209), 1), ((17, 4, 4, 16), 4), ((400, 2, 2, 8), 2),
+    # more samples than blocks; samples of one block an SM and of two
+    ((1500, 3, 5, 12), 3), ((9, 40, 50, 24), 6), ((160, 30, 31, 24), 4),
 ]
 
 
@@ -252,6 +254,24 @@ def test_needed_gradients_only(cuda):
     wh = w.half().requires_grad_(True)
     (gh,) = torch.autograd.grad(dr.group_norm(x, 5, wh, b), (wh,), dy)
     assert gh.dtype == torch.float16
+
+
+def test_more_samples_than_a_grid_counts(cuda):
+    """Over 65535 samples: resident, and (table gradients only) in rounds."""
+    torch = _torch()
+    from opendressi_b200 import ops
+
+    x, dy, w, b = make(17, (70001, 3, 8), torch.float32)
+    y, mean, rstd = ops.group_norm(x, 2, w, b, activation="silu", stats=True)
+    ref = reference(x, w, b, 2, 1e-5, "silu", dy)
+    check(y, ref, "y")
+    for want in ((True, True, True), (False, True, True)):
+        dx, dw, db = ops.group_norm_grad(dy, x, 2, w, b, mean, rstd,
+                                         activation="silu", want=want)
+        if want[0]:
+            check(dx, ref, "dx")
+        check(dw, ref, "dweight")
+        check(db, ref, "dbias")
 
 
 @pytest.mark.parametrize("shape", [(0, 4, 4, 8), (3, 0, 4, 8), (2, 0, 8)])

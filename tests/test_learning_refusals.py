@@ -144,6 +144,9 @@ def adamw_desc(keep, **kw):
     (dict(steps=array("Q", [0])), "null step"),
     (dict(params=array("Q", [1 << 20 | 2])), "aligned"),
     (dict(exp_avg=array("Q", [1 << 20 | 1])), "aligned"),
+    (dict(state_bits=8, exp_avg_sq_scale=array("Q", [1 << 20 | 2])),
+     "aligned"),
+    (dict(steps=array("Q", [1 << 20 | 2])), "null step"),
 ])
 def test_adamw_descriptor(kw, text):
     keep = []
