@@ -721,7 +721,7 @@ void launch_adamw(const AdamWArgs& a, const AdamWHyper& h, uint32_t i0,
 
 template <typename T, int BITS>
 void adamw_t(const AdamWArgs& a, const AdamWHyper& h, cudaStream_t s) {
-    constexpr uint32_t kFew = 32, kSome = 128, kMany = 400;
+    constexpr uint32_t kFew = 32, kSome = 192, kMany = 400;
     for (uint32_t i0 = 0; i0 < a.n_tensors;) {
         // behind the norm's launch, which lets it
         const bool early = h.norm && i0 == 0;
