@@ -10,10 +10,12 @@
 //
 // All of it is bound by memory: 2 values moved per value forward, 3 backward,
 // if what the statistics pass reads is still on chip when the second pass
-// wants it. Statistics are 32-bit per thread about the thread's own first
-// value (no cancellation where |mean| >> deviation) and merged in 64 bits by
-// the pairwise update of Chan, Golub and LeVeque; sums are taken in a fixed
-// order, so reruns give the same bits.
+// wants it (8x256x256x64 bf16 forward: 45 us, against 20.5 for its bytes at the
+// copy rate; 2x1024x1024x64 bf16 with its gradient: 412 us, a sample being
+// larger than L2). Statistics are 32-bit per thread about the thread's own
+// first value (no cancellation where |mean| >> deviation), merged in 32 bits
+// within a block as distances from a common value and in 64 bits between
+// blocks; sums are taken in a fixed order, so reruns give the same bits.
 //
 // Mapping. A thread owns VEC consecutive values and steps by a multiple of a
 // whole row, so it meets the same channels in every step and keeps its sums
@@ -41,7 +43,7 @@ constexpr int kGnResident = 4;      // resident blocks an SM, forward
 constexpr int kGnResidentGrad = 2;  // backward
 
 struct GnDims {
-    uint64_t n, rows;
+    uint64_t rows;
     int C, G, cpg;
     float eps;
     // mapping
@@ -276,8 +278,9 @@ __device__ __forceinline__ void copy_16(void* to, const void* from) {
 }
 
 // Calls ready() once the first loads are under way, then fn(a, b) for `steps`
-// vectors of one image (q null) or two. Whole vectors come through a ring in shared memory, each thread's its own: loads
-// into registers would be a quarter as many.
+// vectors of one image (q null) or two. Whole vectors come through a ring in
+// shared memory, each thread's its own: loads into registers would be a quarter
+// as many.
 template <typename T, int VEC, int IMAGES, typename R, typename F>
 __device__ __forceinline__ void walk_over(const T* p, const T* q,
                                           uint64_t step, uint32_t steps,
@@ -392,11 +395,11 @@ __device__ __forceinline__ Two act_grad2(Two dy, Two z) {
 // Statistics of one (sample, chunk, slab): part[n][g][chunk * pieces + piece]
 // = (mean, sum of squares about it). A thread sums distances from its own
 // first value; runs of `run` channels of a group are merged in the thread, the
-// threads' results by a warp a group: the group's mean is an average of
+// threads' results by some lanes a group: the group's mean is an average of
 // theirs, its sum of squares theirs plus count times (their mean - the mean)^2
 // (the pairwise update of Chan, Golub and LeVeque, all at once). Means enter
-// as distances from one of them: of 1e4 deviations they keep no digits of the
-// variance in 32 bits.
+// as distances from one of them: the square of a mean of many deviations would
+// leave no digits of the variance in 32 bits.
 template <int VEC>
 struct ThreadMoments {
     static constexpr int P = kPairs<VEC>;
@@ -1194,7 +1197,6 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     const int es = a.dtype == 0 ? 4 : 2;
     GnPlan p{};
     GnDims& d = p.d;
-    d.n = a.n;
     d.rows = a.rows;
     d.C = a.C;
     d.G = a.G;
@@ -1391,8 +1393,9 @@ void backward_a(const GnPlan& p, const GroupNormArgs& a, const void* dy,
     };
     if (p.items) {
         launch(k_gn_resident_grad<T, VEC, ACT>, dim3(p.grid), p.smem, false, s,
-               p.d, p.items, static_cast<const T*>(dy), static_cast<const T*>(x),
-               weight, bias, mean, rstd, w.sums, static_cast<T*>(dx));
+               p.d, p.items, static_cast<const T*>(dy),
+               static_cast<const T*>(x), weight, bias, mean, rstd, w.sums,
+               static_cast<T*>(dx));
         affine(a.n);
         return;
     }
