@@ -71,6 +71,12 @@ Tensor bytes_on(const Tensor& like, size_t n) {
     return at::empty({int64_t(n)}, like.options().dtype(at::kByte));
 }
 
+// Tells autograd that t's values were written: a graph that has kept the ones
+// before refuses its backward pass.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 const float* floats(const Tensor& t) {
     return t.defined() ? static_cast<const float*>(t.const_data_ptr())
                        : nullptr;
@@ -283,6 +289,7 @@ void norm_of(const Addresses& a, const Tensor& out) {
                           static_cast<float*>(out.mutable_data_ptr()),
                           space.mutable_data_ptr(), need, stream_of(out)),
          "grad_norm");
+    written(out);
 }
 
 Tensor grad_norm(const std::vector<Tensor>& tensors,
@@ -314,6 +321,7 @@ Tensor grad_norm(const std::vector<Tensor>& tensors,
         if (out.scalar_type() != at::kFloat || out.numel() != 1 ||
             out.device() != dev)
             refuse("out must hold one float32 on " + dev.str());
+        if (out.requires_grad()) refuse("out requires a gradient");
     } else {
         out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
     }
@@ -338,13 +346,15 @@ struct Pack {
         uint32_t index;
     };
     std::vector<Row> rows;
+    std::vector<Tensor> state;  // what the rows' addresses are in
     int32_t state_bits;
 
     Pack(const std::vector<Tensor>& params, const std::vector<int64_t>& blocks,
          const Tensor& step, const Tensor& m, const Tensor& v,
          const optional<Tensor>& sm, const optional<Tensor>& sv,
          int64_t index, int64_t bits)
-        : state_bits(int32_t(bits)) {
+        : state{step, m, v}, state_bits(int32_t(bits)) {
+        if (bits == 8) state.insert(state.end(), {*sm, *sv});
         for (size_t i = 0; i < params.size(); i++) {
             Row r;
             r.p = params[i];
@@ -446,6 +456,9 @@ struct Pack {
             d.seed = uint32_t(seed);
             d.ticket = static_cast<uint32_t*>(ticket.mutable_data_ptr());
             done(dressi_adamw_step(&d, stream_of(ticket)), "adamw");
+            for (const Row& r : rows)
+                if (r.dtype == dtype && r.g.defined()) written(r.p);
+            for (const Tensor& t : state) written(t);
         }
     }
 };

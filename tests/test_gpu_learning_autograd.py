@@ -1,0 +1,75 @@
+"""What autograd, forward mode and tracing see of the learning operators."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def leaves(*shapes, dtype=None):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    return [torch.nn.Parameter(torch.randn(s, generator=g, device="cuda")
+                               .to(dtype or torch.float32)) for s in shapes]
+
+
+# ------------------------------------------------------------------ versions
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_graph_of_the_values_before_a_step_is_refused(cuda, dtype, bits):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    p, q = leaves((300,), (7, 5), dtype=getattr(torch, dtype))
+    opt = optim.AdamW([p, q], state_bits=bits)
+    loss = (p * p).sum() + (q * q).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_versions_grow_where_a_step_writes(cuda, bits):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    a, late, b = leaves((300,), (9,), (33, 4))
+    (h,) = leaves((70,), dtype=torch.float16)
+    opt = optim.AdamW([{"params": [a, late]}, {"params": [b, h]}],
+                      state_bits=bits, max_norm=1.0)
+    for p in (a, b, h):
+        p.grad = torch.ones_like(p)
+    watched = {"last_norm": opt.last_norm}
+    for g in range(2):
+        for k, t in opt.packed_state(g).items():
+            watched[k, g] = t
+    watched["a"], watched["b"], watched["h"] = a, b, h
+    watched["view"] = opt.state[a]["exp_avg"]
+    before = {k: t._version for k, t in watched.items()}
+    kept = late._version, a.grad._version
+    opt.step()
+    for k, t in watched.items():
+        assert t._version > before[k], k
+    assert (late._version, a.grad._version) == kept
+
+
+def test_norm_into_a_tensor_that_a_graph_keeps(cuda):
+    torch = _torch()
+    from opendressi_b200 import DressiError, optim
+
+    (p,) = leaves((300,))
+    out = torch.ones((), device="cuda")
+    w = torch.ones((), device="cuda", requires_grad=True)
+    kept = w * out
+    got = optim.grad_norm([p], out=out)
+    assert got.data_ptr() == out.data_ptr() and not got.requires_grad
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        kept.backward()
+    with pytest.raises(DressiError, match="requires a gradient"):
+        optim.grad_norm([p], out=w)
