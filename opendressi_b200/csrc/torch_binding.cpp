@@ -4,6 +4,7 @@
 // training step: a group norm's forward and backward cost 166 us of host time
 // through Python and ctypes, and a step over 150 tensors 300 us, several times
 // what their kernels take.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -250,17 +251,27 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     }
 };
 
+// Whether t carries a tangent that forward-mode differentiation expects a
+// result to carry on.
+bool has_tangent(const Tensor& t) {
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+           t._fw_grad(/*level=*/0).defined();
+}
+
 Tensor group_norm(const Tensor& x, int64_t groups,
                   optional<Tensor> weight, optional<Tensor> bias, double eps,
                   const std::string& activation) {
     const int act = activation_of(activation);
-    bool grad = x.requires_grad();
+    bool grad = x.requires_grad(), tangent = has_tangent(x);
     for (optional<Tensor>* t : {&weight, &bias})
         if (t->has_value()) {
+            tangent |= has_tangent(**t);
             on_cuda(**t, t == &weight ? "weight" : "bias");
             *t = (*t)->to(at::kFloat);
             grad |= (*t)->requires_grad();
         }
+    // dropped, it would read as a derivative of zero
+    if (tangent) refuse("group_norm has no forward-mode derivative");
     if (grad && at::GradMode::is_enabled())
         return GroupNorm::apply(x, groups, weight, bias, eps, int64_t(act));
     return norm_forward(x, groups, weight.value_or(Tensor()),

@@ -720,7 +720,8 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
     ("none", "relu" or "silu"). x is float32, float16 or bfloat16 and so is
     the result; statistics are taken in 32 bits and more. A channels-last
     tensor of shape [N, C, H, W] is given as x.permute(0, 2, 3, 1), which
-    copies nothing. Differentiable once, w.r.t. x, weight and bias."""
+    copies nothing. Differentiable once, w.r.t. x, weight and bias, in reverse
+    mode (an input with a forward-mode tangent is refused)."""
     if torch.compiler.is_compiling():
         weight = None if weight is None else weight.to(torch.float32)
         bias = None if bias is None else bias.to(torch.float32)

@@ -73,3 +73,40 @@ def test_norm_into_a_tensor_that_a_graph_keeps(cuda):
         kept.backward()
     with pytest.raises(DressiError, match="requires a gradient"):
         optim.grad_norm([p], out=w)
+
+
+# -------------------------------------------------------------- forward mode
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias"])
+@pytest.mark.parametrize("with_grad", [False, True])
+def test_forward_mode_is_refused(cuda, which, with_grad):
+    """A tangent is not dropped, which would read as a derivative of zero."""
+    torch = _torch()
+    import torch.autograd.forward_ad as fw
+
+    from opendressi_b200 import torch_api as dr
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((2, 5, 4, 8), generator=g, device="cuda")
+    args = {"x": x, "weight": torch.ones(8, device="cuda"),
+            "bias": torch.zeros(8, device="cuda")}
+    clean = dr.group_norm(num_groups=2, **args)
+    with fw.dual_level():
+        primal = args[which].clone().requires_grad_(with_grad)
+        dual = fw.make_dual(primal, torch.ones_like(primal))
+        with pytest.raises(RuntimeError, match="forward"):
+            dr.group_norm(num_groups=2, **{**args, which: dual})
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+            dr.group_norm(num_groups=2, **{**args, which: dual})
+        # where tangents are switched off none is expected
+        with fw._set_fwd_grad_enabled(False):
+            y = dr.group_norm(num_groups=2, **{**args, which: dual})
+        assert torch.equal(y, clean)
+        # a call without one inside a dual level
+        assert torch.equal(dr.group_norm(num_groups=2, **args), clean)
+
+    def f(t):
+        return dr.group_norm(num_groups=2, **{**args, which: t})
+
+    with pytest.raises(RuntimeError, match="forward"):
+        torch.func.jvp(f, (args[which],), (torch.ones_like(args[which]),))
