@@ -5,6 +5,7 @@
 // through Python and ctypes, and a step over 150 tensors 300 us, several times
 // what their kernels take.
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -258,20 +259,47 @@ bool has_tangent(const Tensor& t) {
            t._fw_grad(/*level=*/0).defined();
 }
 
-Tensor group_norm(const Tensor& x, int64_t groups,
-                  optional<Tensor> weight, optional<Tensor> bias, double eps,
-                  const std::string& activation) {
+// Whether something looks at the operators of this thread as they are called
+// (a tracer, a dispatch mode, a transform), or t stands for other values than
+// its memory holds (a subclass, a transform's wrapper, a lazy negation). What
+// is computed past the dispatcher would be missing from a trace.
+bool dispatched() {
+    for (const auto k :
+         {c10::DispatchKey::Python, c10::DispatchKey::PythonDispatcher,
+          c10::DispatchKey::Tracer, c10::DispatchKey::Functionalize,
+          c10::DispatchKey::FuncTorchDynamicLayerFrontMode})
+        if (c10::impl::tls_is_dispatch_key_included(k)) return true;
+    return false;
+}
+bool dispatched(const Tensor& t) {
+    return t.key_set().has_any(c10::DispatchKeySet(
+            {c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
+             c10::DispatchKey::FuncTorchBatched,
+             c10::DispatchKey::FuncTorchGradWrapper,
+             c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor}));
+}
+
+// None where the call has to go through the dispatcher.
+optional<Tensor> group_norm(const Tensor& x, int64_t groups,
+                            optional<Tensor> weight, optional<Tensor> bias,
+                            double eps, const std::string& activation) {
     const int act = activation_of(activation);
     bool grad = x.requires_grad(), tangent = has_tangent(x);
-    for (optional<Tensor>* t : {&weight, &bias})
+    bool dispatch = dispatched() || dispatched(x);
+    for (const optional<Tensor>* t : {&weight, &bias})
         if (t->has_value()) {
             tangent |= has_tangent(**t);
+            dispatch |= dispatched(**t);
+        }
+    // dropped, it would read as a derivative of zero
+    if (tangent) refuse("group_norm has no forward-mode derivative");
+    if (dispatch) return c10::nullopt;
+    for (optional<Tensor>* t : {&weight, &bias})
+        if (t->has_value()) {
             on_cuda(**t, t == &weight ? "weight" : "bias");
             *t = (*t)->to(at::kFloat);
             grad |= (*t)->requires_grad();
         }
-    // dropped, it would read as a derivative of zero
-    if (tangent) refuse("group_norm has no forward-mode derivative");
     if (grad && at::GradMode::is_enabled())
         return GroupNorm::apply(x, groups, weight, bias, eps, int64_t(act));
     return norm_forward(x, groups, weight.value_or(Tensor()),

@@ -722,11 +722,14 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
     tensor of shape [N, C, H, W] is given as x.permute(0, 2, 3, 1), which
     copies nothing. Differentiable once, w.r.t. x, weight and bias, in reverse
     mode (an input with a forward-mode tangent is refused)."""
-    if torch.compiler.is_compiling():
-        weight = None if weight is None else weight.to(torch.float32)
-        bias = None if bias is None else bias.to(torch.float32)
-        return _group_norm_op(x, weight, bias, num_groups, float(eps),
-                              activation)[0]
-    # outside of a trace the same calls with their autograd in C++
-    return ops.binding().group_norm(x, num_groups, weight, bias, eps,
-                                    activation)
+    if not torch.compiler.is_compiling():
+        # the operator below with its autograd in C++, unless a trace or a
+        # transform has to see it
+        y = ops.binding().group_norm(x, num_groups, weight, bias, eps,
+                                     activation)
+        if y is not None:
+            return y
+    weight = None if weight is None else weight.to(torch.float32)
+    bias = None if bias is None else bias.to(torch.float32)
+    return _group_norm_op(x, weight, bias, num_groups, float(eps),
+                          activation)[0]

@@ -110,3 +110,98 @@ def test_forward_mode_is_refused(cuda, which, with_grad):
 
     with pytest.raises(RuntimeError, match="forward"):
         torch.func.jvp(f, (args[which],), (torch.ones_like(args[which]),))
+
+
+# ------------------------------------------------------------------- tracing
+
+def inputs(seed):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*s):
+        return torch.randn(s, generator=g, device="cuda")
+
+    return normal(2, 9, 7, 12) + 1, 1 + normal(12) / 4, normal(12)
+
+
+def norm(x, w, b):
+    from opendressi_b200 import torch_api as dr
+
+    return dr.group_norm(x * 2.0, 3, w, b, activation="silu") + 1.0
+
+
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+def test_traced_by_make_fx(cuda, mode):
+    torch = _torch()
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    traced = make_fx(norm, tracing_mode=mode)(*inputs(1))
+    assert any("dressi_b200.group_norm" in str(n.target)
+               for n in traced.graph.nodes)
+    new = inputs(2)
+    torch.empty(1 << 20, device="cuda").fill_(7.0)  # what memory held before
+    assert torch.equal(traced(*new), norm(*new))
+
+
+def test_traced_by_jit(cuda):
+    torch = _torch()
+    with torch.no_grad():
+        traced = torch.jit.trace(norm, inputs(1))
+        assert "dressi_b200::group_norm" in str(traced.graph)
+        new = inputs(2)
+        assert torch.equal(traced(*new), norm(*new))
+
+
+def test_functional_transforms(cuda):
+    """vmap takes sample after sample; grad is refused."""
+    torch = _torch()
+    x, w, b = inputs(3)
+    xs = torch.stack([x, x + 1.0, -x])
+    got = torch.vmap(lambda t: norm(t, w, b))(xs)
+    assert torch.equal(got, torch.stack([norm(t, w, b) for t in xs]))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: norm(t, w, b).square().sum())(x)
+
+
+def test_a_dispatch_mode_sees_the_operator(cuda):
+    torch = _torch()
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    args = inputs(5)
+    with Log():
+        y = norm(*args)
+    assert any("dressi_b200.group_norm" in s for s in seen)
+    assert torch.equal(y, norm(*args))
+
+
+def test_selective_recomputation(cuda):
+    """Checkpointing that keeps some operators' results runs under a dispatch
+    mode: what it recomputes is computed."""
+    torch = _torch()
+    from torch.utils import checkpoint as ck
+
+    def policy(ctx, op, *a, **k):
+        return (ck.CheckpointPolicy.MUST_SAVE if "empty" in str(op)
+                else ck.CheckpointPolicy.PREFER_RECOMPUTE)
+
+    x, w, b = inputs(6)
+
+    def f(x, w, b):
+        return norm(norm(x, w, b), w, b)
+
+    def gradients(call):
+        ts = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        return torch.autograd.grad(call(*ts).square().sum(), ts)
+
+    got = gradients(lambda *t: ck.checkpoint(
+        f, *t, use_reentrant=False,
+        context_fn=lambda: ck.create_selective_checkpoint_contexts(policy)))
+    for a, e in zip(got, gradients(f)):
+        assert torch.equal(a, e)
