@@ -6,6 +6,7 @@
 // what their kernels take.
 #include <c10/core/AutogradState.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -306,6 +307,20 @@ optional<Tensor> group_norm(const Tensor& x, int64_t groups,
                         bias.value_or(Tensor()), eps, act, false)[0];
 }
 
+// ------------------------------------------------------------------- traces
+
+// The norm and the step below are no operators that a trace could hold: it
+// would be left without their result, and without what they write. Modes that
+// look on while real tensors are computed are welcome.
+void not_traced(const char* what) {
+    using Mode = c10::impl::TorchDispatchModeKey;
+    bool traced =
+            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer);
+    for (const auto k : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL})
+        traced |= c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
+    if (traced) refuse(std::string(what) + " cannot be traced");
+}
+
 // --------------------------------------------------------------------- norm
 
 struct Addresses {
@@ -333,6 +348,7 @@ void norm_of(const Addresses& a, const Tensor& out) {
 
 Tensor grad_norm(const std::vector<Tensor>& tensors,
                  const optional<Tensor>& out_) {
+    not_traced("grad_norm");
     at::NoGradGuard none;
     Addresses a;
     std::vector<Tensor> held;  // copies of what is not contiguous
@@ -510,6 +526,7 @@ void adamw_step(const std::vector<Pack*>& packs,
                 const std::vector<Numbers>& numbers, double max_norm,
                 const optional<Tensor>& norm, int64_t seed,
                 const Tensor& ticket) {
+    not_traced("an AdamW step");
     const c10::cuda::CUDAGuard guard(ticket.device());
     struct Release {
         const std::vector<Pack*>& packs;

@@ -4,7 +4,8 @@ The counterpart, for a torch program, of the Adam inside the fused plans
 (which steps one flat parameter): one kernel launch steps the vertices,
 textures, material maps and network weights of a scene. The step runs on the
 parameters' device and its current stream, reads nothing back and keeps its
-counters on the device, so it can be captured in a CUDA graph.
+counters on the device, so it can be captured in a CUDA graph. It is no
+operator of a torch graph: make_fx and torch.jit.trace refuse it.
 """
 
 from __future__ import annotations

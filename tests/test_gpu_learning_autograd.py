@@ -205,3 +205,37 @@ def test_selective_recomputation(cuda):
         context_fn=lambda: ck.create_selective_checkpoint_contexts(policy)))
     for a, e in zip(got, gradients(f)):
         assert torch.equal(a, e)
+
+
+def test_norm_and_step_refuse_a_trace(cuda):
+    """Their result is not a value of the trace, and their writes no part of
+    it: better refused than left out."""
+    torch = _torch()
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from opendressi_b200 import DressiError, optim
+
+    (p,) = leaves((300,))
+    p.grad = torch.ones_like(p)
+    opt = optim.AdamW([p])
+    before = p.detach().clone()
+
+    def step(t):
+        opt.step()
+        return t + 1.0
+
+    for trace in (lambda f: make_fx(f)(p.grad),
+                  lambda f: torch.jit.trace(f, (p.grad,))):
+        with pytest.raises(DressiError, match="traced"):
+            trace(lambda t: optim.grad_norm([t]) + 1.0)
+        with pytest.raises(DressiError, match="traced"):
+            trace(step)
+    assert torch.equal(p, before)
+    assert int(opt.state[p]["step"]) == 0
+    # other dispatch modes look on
+    from torch.utils.flop_counter import FlopCounterMode
+
+    with FlopCounterMode(display=False):
+        opt.step()
+        n = optim.grad_norm([p.grad])
+    assert int(opt.state[p]["step"]) == 1 and float(n) > 17.3
