@@ -10,6 +10,7 @@ operator of a torch graph: make_fx and torch.jit.trace refuse it.
 
 from __future__ import annotations
 
+import copy
 import math
 
 import torch
@@ -236,10 +237,23 @@ class AdamW(torch.optim.Optimizer):
                        "max_norm": self.max_norm}
         return sd
 
+    @staticmethod
+    def _loaded_options(group, saved) -> dict:
+        """A group's options with copies of the saved ones in their place."""
+        options = {k: v.detach().clone() if isinstance(v, torch.Tensor)
+                   else copy.deepcopy(v)
+                   for k, v in saved.items() if k != "params"}
+        return {**group, **options}
+
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """Copies a state_dict() of an optimizer over like parameters into
-        this one's own tensors."""
+        this one's own tensors (a learning rate that is a tensor here among
+        them, so that a captured step reads the loaded one)."""
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            if changed is not None:
+                state_dict = changed
         own = state_dict.get("adamw", {})
         if own.get("state_bits") != self.state_bits:
             raise ValueError("the state was kept in "
@@ -259,11 +273,18 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f"the state's {kind} is not like "
                                          "this optimizer's")
                     pairs.append((t, got[kind]))
-        for group, old in zip(self.param_groups, groups):
-            merged = {**group, **{k: v for k, v in old.items()
-                                  if k != "params"}}
-            self._check_options(merged)
-            group.update(merged)
+        options = [self._loaded_options(g, old)
+                   for g, old in zip(self.param_groups, groups)]
+        for new in options:  # all of it is right before any is changed
+            self._check_options({**new, "lr": float(new["lr"])})
+        for group, new in zip(self.param_groups, options):
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor):
+                lr.copy_(torch.as_tensor(new["lr"]).reshape(lr.shape))
+                new["lr"] = lr
+            elif isinstance(new["lr"], torch.Tensor) and new["lr"].is_cuda:
+                new["lr"] = new["lr"].to(self._device, torch.float32)
+            group.update(new)
         for t, got in pairs:
             t.copy_(got)
         self.seed = int(own.get("seed", self.seed))
@@ -272,6 +293,8 @@ class AdamW(torch.optim.Optimizer):
                 self._device is not None:
             self.last_norm = torch.zeros((), dtype=torch.float32,
                                          device=self._device)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def __getstate__(self):
         raise TypeError("an AdamW holds device state: save its state_dict()")

@@ -1,0 +1,126 @@
+"""AdamW's options and tensors where a program changes them between steps."""
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def leaves(*shapes):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(8)
+    out = [torch.nn.Parameter(torch.randn(s, generator=g, device="cuda"))
+           for s in shapes]
+    for p in out:
+        p.grad = torch.randn(p.shape, generator=g, device="cuda")
+    return out
+
+
+def tensor_lr(value):
+    return _torch().tensor(value, device="cuda")
+
+
+# ---------------------------------------------------------- loaded options
+
+def test_loading_shares_no_learning_rate(cuda):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    a = optim.AdamW(leaves((9,)), lr=tensor_lr(0.125))
+    b = optim.AdamW(leaves((9,)), lr=tensor_lr(0.5))
+    c = optim.AdamW(leaves((9,)), lr=0.5, clamp=[0.0, 1.0])
+    own = b.param_groups[0]["lr"]
+    b.load_state_dict(a.state_dict())
+    c.load_state_dict(a.state_dict())
+    assert b.param_groups[0]["lr"] is own and float(own) == 0.125
+    got = c.param_groups[0]["lr"]
+    assert got.is_cuda and float(got) == 0.125
+    a.param_groups[0]["lr"].fill_(0.25)
+    assert float(own) == 0.125 and float(got) == 0.125
+    # a number into a tensor, a CPU copy into a tensor, a list is copied
+    number = optim.AdamW(leaves((9,)), lr=0.0625, clamp=[0.0, 2.0])
+    b.load_state_dict(number.state_dict())
+    assert b.param_groups[0]["lr"] is own and float(own) == 0.0625
+    assert b.param_groups[0]["clamp"] == [0.0, 2.0]
+    assert b.param_groups[0]["clamp"] is not number.param_groups[0]["clamp"]
+    state = a.state_dict()
+    state["param_groups"][0]["lr"] = torch.tensor(0.75, dtype=torch.float64)
+    b.load_state_dict(state)
+    assert b.param_groups[0]["lr"] is own and float(own) == 0.75
+
+
+@pytest.mark.parametrize("bad", [-1.0, math.nan, math.inf])
+def test_a_refused_load_changes_nothing(cuda, bad):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    a = optim.AdamW(leaves((9,), (4,)), lr=tensor_lr(0.125))
+    a.step()
+    b = optim.AdamW([{"params": p} for p in leaves((9,), (4,))], lr=0.5)
+    one = optim.AdamW([{"params": p} for p in leaves((9,), (4,))], lr=0.25)
+    one.step()
+    for lr in (bad, torch.tensor(bad)):
+        state = one.state_dict()
+        state["param_groups"][1]["lr"] = lr
+        with pytest.raises(ValueError):
+            b.load_state_dict(state)
+        assert [g["lr"] for g in b.param_groups] == [0.5, 0.5]
+        assert not b.packed_state()["exp_avg"].any()
+
+
+def test_a_captured_step_reads_a_loaded_learning_rate(cuda):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    pa, pb = leaves((700,), (3, 5)), leaves((700,), (3, 5))
+    a = optim.AdamW(pa, lr=tensor_lr(2.0 ** -7))
+    b = optim.AdamW(pb, lr=2.0 ** -7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a.step()
+    torch.cuda.current_stream().wait_stream(side)
+    b.step()
+    saved = b.state_dict()
+    saved["param_groups"][0]["lr"] = 2.0 ** -4
+    saved = {**saved, "state": {k: {n: t.clone() for n, t in v.items()}
+                                for k, v in saved["state"].items()}}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    a.load_state_dict(saved)
+    b.load_state_dict(saved)
+    graph.replay()
+    b.step()
+    a.param_groups[0]["lr"].fill_(2.0 ** -3)
+    b.param_groups[0]["lr"] = 2.0 ** -3
+    graph.replay()
+    b.step()
+    for x, y in zip(pa, pb):
+        assert torch.equal(x, y)
+
+
+def test_load_hooks_run(cuda):
+    from opendressi_b200 import optim
+
+    a, b = optim.AdamW(leaves((9,)), lr=0.125), optim.AdamW(leaves((9,)))
+    seen = []
+
+    def before(opt, state):
+        seen.append("before")
+        state = dict(state)
+        state["param_groups"] = [{**g, "lr": 0.75}
+                                 for g in state["param_groups"]]
+        return state
+
+    b.register_load_state_dict_pre_hook(before)
+    b.register_load_state_dict_post_hook(lambda opt: seen.append(
+        opt.param_groups[0]["lr"]))
+    b.load_state_dict(a.state_dict())
+    assert seen == ["before", 0.75]
