@@ -392,7 +392,7 @@ struct Pack {
         Tensor p, g;
         int32_t dtype;
         uint64_t n;
-        std::vector<int64_t> strides;
+        std::vector<int64_t> sizes, strides;
         void* m;
         void* v;
         float* sm;
@@ -415,6 +415,7 @@ struct Pack {
             r.p = params[i];
             r.dtype = dtype_of(r.p, "parameter");
             r.n = uint64_t(r.p.numel());
+            r.sizes = r.p.sizes().vec();
             r.strides = r.p.strides().vec();
             const int64_t at = blocks[i] * 256 * m.element_size();
             r.m = static_cast<char*>(m.mutable_data_ptr()) + at;
@@ -434,8 +435,11 @@ struct Pack {
     void gather(const at::Device& dev) {
         at::NoGradGuard none;
         for (Row& r : rows) {
+            // as many values and the same strides could still be a view that
+            // is not dense: the kernel writes numel values in a row
             if (dtype_of(r.p, "parameter") != r.dtype ||
-                uint64_t(r.p.numel()) != r.n || r.p.device() != dev ||
+                r.p.device() != dev ||
+                r.p.sizes() != at::IntArrayRef(r.sizes) ||
                 r.p.strides() != at::IntArrayRef(r.strides)) {
                 refuse("a parameter changed its type, shape or device; make a "
                        "new optimizer");

@@ -124,3 +124,33 @@ def test_load_hooks_run(cuda):
         opt.param_groups[0]["lr"]))
     b.load_state_dict(a.state_dict())
     assert seen == ["before", 0.75]
+
+
+# ------------------------------------------------------- changed parameters
+
+def test_a_parameter_of_another_shape_is_refused(cuda):
+    """Also one with as many values and the same strides, which are then no
+    longer dense: (3, 2) cut out of (3, 3), or one value as six."""
+    torch = _torch()
+    from opendressi_b200 import DressiError, optim
+
+    wide = torch.randn(3, 3, device="cuda")
+    p = torch.nn.Parameter(torch.randn(2, 3, device="cuda"))
+    opt = optim.AdamW([p])
+    p.data = wide[:, :2]
+    p.grad = torch.ones_like(p)
+    assert p.stride() == (3, 1) and p.numel() == 6
+    before = wide.clone()
+    with pytest.raises(DressiError, match="changed"):
+        opt.step()
+    row = torch.randn(1, 6, device="cuda").as_strided((1, 6), (0, 1))
+    q = torch.nn.Parameter(row)
+    opt = optim.AdamW([q])
+    one = torch.randn(8, device="cuda")
+    q.data = one[:1].as_strided((6, 1), (0, 1))
+    q.grad = torch.ones(6, 1, device="cuda")
+    assert q.numel() == 6
+    kept = one.clone()
+    with pytest.raises(DressiError, match="changed"):
+        opt.step()
+    assert torch.equal(wide, before) and torch.equal(one, kept)
