@@ -172,14 +172,18 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("parameters share memory")
         super().add_param_group(group)
         params = self.param_groups[-1]["params"]
-        if dev is not None and self._device is None:
-            self._device = dev
-            self._ticket = torch.zeros(1, dtype=torch.int32, device=dev)
-            if self.max_norm is not None:
-                self.last_norm = torch.zeros((), dtype=torch.float32,
-                                             device=dev)
-        pack = _Pack(params, self.state_bits,
-                     sum(len(q.params) for q in self._packs))
+        try:
+            if dev is not None and self._device is None:
+                self._ticket = torch.zeros(1, dtype=torch.int32, device=dev)
+                if self.max_norm is not None:
+                    self.last_norm = torch.zeros((), dtype=torch.float32,
+                                                 device=dev)
+            pack = _Pack(params, self.state_bits,
+                         sum(len(q.params) for q in self._packs))
+        except BaseException:  # groups and packs go together
+            self.param_groups.pop()
+            raise
+        self._device = dev
         self._packs.append(pack)
         for p, view in zip(params, pack.views):
             self.state[p] = view

@@ -154,3 +154,26 @@ def test_a_parameter_of_another_shape_is_refused(cuda):
     with pytest.raises(DressiError, match="changed"):
         opt.step()
     assert torch.equal(wide, before) and torch.equal(one, kept)
+
+
+def test_a_group_that_fails_to_be_added_leaves_no_trace(cuda, monkeypatch):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    p, q, r = leaves((9,), (4,), (5,))
+    opt = optim.AdamW([p], lr=0.5)
+
+    def full(*args, **kw):
+        raise torch.OutOfMemoryError("no memory for the state")
+
+    with monkeypatch.context() as m:
+        m.setattr(optim, "_Pack", full)
+        with pytest.raises(torch.OutOfMemoryError):
+            opt.add_param_group({"params": [q], "lr": 0.25})
+    assert len(opt.param_groups) == 1 and q not in opt.state
+    opt.add_param_group({"params": [r], "lr": 0.0, "weight_decay": 0.0})
+    opt.add_param_group({"params": [q], "lr": 0.25})
+    before = [t.detach().clone() for t in (p, q, r)]
+    opt.step()
+    assert not torch.equal(p, before[0]) and not torch.equal(q, before[1])
+    assert torch.equal(r, before[2])  # its own learning rate
