@@ -125,7 +125,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("lr must be a number or hold one")
             if lr.is_cuda and lr.dtype != torch.float32:
                 raise ValueError("a CUDA lr must be float32")
-        elif not 0.0 <= lr < math.inf:
+            lr = 0.0 if lr.is_cuda else float(lr)  # no read from the device
+        if not 0.0 <= lr < math.inf:
             raise ValueError(f"lr must be finite and not negative, got {lr}")
         if len(g["betas"]) != 2 or not all(0.0 <= b < 1.0
                                            for b in g["betas"]):

@@ -177,3 +177,18 @@ def test_a_group_that_fails_to_be_added_leaves_no_trace(cuda, monkeypatch):
     opt.step()
     assert not torch.equal(p, before[0]) and not torch.equal(q, before[1])
     assert torch.equal(r, before[2])  # its own learning rate
+
+
+def test_a_host_learning_rate_is_checked_before_any_group_steps(cuda):
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    p, q = leaves((9,), (4,))
+    with pytest.raises(ValueError):
+        optim.AdamW([p], lr=torch.tensor(-1.0))
+    opt = optim.AdamW([{"params": p}, {"params": q}], lr=torch.tensor(0.5))
+    opt.param_groups[1]["lr"] = torch.tensor(math.nan)
+    before = p.detach().clone()
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(p, before) and int(opt.state[p]["step"]) == 0
