@@ -1192,6 +1192,11 @@ void split_rows(GnDims* d, uint64_t chunks, uint64_t row_unit) {
     d->chunks = uint32_t((d->rows + d->chunk_rows - 1) / d->chunk_rows);
 }
 
+// Dynamic shared memory of a resident block where `each` share an SM.
+constexpr uint64_t resident_bytes(int each) {
+    return uint64_t(226 / each - 3) << 10;
+}
+
 GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
                  bool grad, bool resident) {
     const int es = a.dtype == 0 ? 4 : 2;
@@ -1267,7 +1272,7 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     if (resident && d.pieces == 1 && items < (1u << 30)) {
         for (int each = most; each >= 1; each /= 2) {
             const uint64_t bytes = steps * step_bytes + side;
-            if (bytes > uint64_t(226 / each - 3) << 10) continue;
+            if (bytes > resident_bytes(each)) continue;
             if (each < most && items > uint64_t(kGnSms) * each) break;
             split_rows(&d, 1, row_unit);
             d.slots = int(steps);
@@ -1336,12 +1341,16 @@ GnWorkspace carve(const GroupNormArgs& a, const GnPlan& p, bool grad,
 }
 
 // Launches a kernel with `smem` bytes of dynamic shared memory; early: it may
-// begin while the launch before still runs (which is one of this file).
+// begin while the launch before still runs (which is one of this file). What a
+// kernel may use is the kernel's own state, shared by all host threads, so it
+// is always set to the same: the most of any call.
 template <typename... P, typename... A>
 void launch(void (*kernel)(P...), dim3 grid, int smem, bool early,
             cudaStream_t s, A... args) {
-    DRESSI_CUDA(cudaFuncSetAttribute(
-            kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (smem > 40 << 10)  // 48 KB with a kernel's static tables need no leave
+        DRESSI_CUDA(cudaFuncSetAttribute(
+                kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                int(resident_bytes(1))));
     if (early) {
         launch_early(kernel, grid, kGnThreads, size_t(smem), s, args...);
         return;
