@@ -783,10 +783,12 @@ __global__ void __launch_bounds__(kGnThreads, kGnResident)
 
 // ----------------------------------------------------------------- backward
 
-// What a thread's channels are scaled by: -mean, rstd, weight, bias.
+// What a thread's channels are scaled by: -mean, rstd, rstd weight, bias. z is
+// (x - mean) (rstd weight) + bias as in the forward pass, rounded alike: relu
+// passes a gradient exactly where it passed a value.
 template <int VEC>
 struct Scales {
-    Two mu[kPairs<VEC>], r[kPairs<VEC>], wt[kPairs<VEC>], b[kPairs<VEC>];
+    Two mu[kPairs<VEC>], r[kPairs<VEC>], a[kPairs<VEC>], b[kPairs<VEC>];
 };
 template <int VEC>
 __device__ __forceinline__ Scales<VEC> scales_of(const GnDims& d,
@@ -796,23 +798,32 @@ __device__ __forceinline__ Scales<VEC> scales_of(const GnDims& d,
                                                  const float* mean,
                                                  const float* rstd) {
     constexpr int P = kPairs<VEC>;
-    float m1[2 * P], r1[2 * P], w1[2 * P], b1[2 * P];
+    float m1[2 * P], r1[2 * P], a1[2 * P], b1[2 * P];
     each_channel<VEC>(d, w, [&](int j, int c, int g) {
         m1[j] = -mean[n * d.G + g];
         r1[j] = rstd[n * d.G + g];
-        w1[j] = weight ? weight[c] : 1.f;
+        a1[j] = r1[j] * (weight ? weight[c] : 1.f);
         b1[j] = bias ? bias[c] : 0.f;
     });
-    if (VEC == 1) m1[1] = r1[1] = w1[1] = b1[1] = 0.f;
+    if (VEC == 1) m1[1] = r1[1] = a1[1] = b1[1] = 0.f;
     Scales<VEC> s;
 #pragma unroll
     for (int j = 0; j < P; j++) {
         s.mu[j] = two(m1[2 * j], m1[2 * j + 1]);
         s.r[j] = two(r1[2 * j], r1[2 * j + 1]);
-        s.wt[j] = two(w1[2 * j], w1[2 * j + 1]);
+        s.a[j] = two(a1[2 * j], a1[2 * j + 1]);
         s.b[j] = two(b1[2 * j], b1[2 * j + 1]);
     }
     return s;
+}
+
+// (x, dy) of a pair of values to (h, dz).
+template <int ACT, int VEC>
+__device__ __forceinline__ void terms(const Scales<VEC>& c, int j, Two* h,
+                                      Two* g) {
+    const Two e = add2(h[j], c.mu[j]);
+    h[j] = mul2(e, c.r[j]);
+    g[j] = act_grad2<ACT>(g[j], fma2(e, c.a[j], c.b[j]));
 }
 
 // part[n][chunk][c] = (sum dz, sum dz h) over the chunk's rows.
@@ -850,9 +861,7 @@ __global__ void __launch_bounds__(kGnThreads)
                     unpack<T, VEC>(e, g);
 #pragma unroll
                     for (int j = 0; j < P; j++) {
-                        h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
-                        g[j] = act_grad2<ACT>(g[j],
-                                              fma2(h[j], c.wt[j], c.b[j]));
+                        terms<ACT>(c, j, h, g);
                         A[j] = add2(A[j], g[j]);
                         B[j] = fma2(g[j], h[j], B[j]);
                     }
@@ -964,8 +973,9 @@ __global__ void __launch_bounds__(kGnThreads)
         float a1[2 * P], b1[2 * P];
         each_channel<VEC>(d, w, [&](int j, int, int g) {
             const float2 m = means[n * d.G + g];
-            a1[j] = -m.x;
-            b1[j] = -m.y;
+            const float r = rstd[n * d.G + g];
+            a1[j] = -m.x * r;
+            b1[j] = -m.y * r;
         });
         if (VEC == 1) a1[1] = b1[1] = 0.f;
 #pragma unroll
@@ -984,10 +994,8 @@ __global__ void __launch_bounds__(kGnThreads)
                 unpack<T, VEC>(e, g);
 #pragma unroll
                 for (int j = 0; j < P; j++) {
-                    h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
-                    g[j] = act_grad2<ACT>(g[j], fma2(h[j], c.wt[j], c.b[j]));
-                    g[j] = mul2(c.r[j], fma2(h[j], mb[j],
-                                             fma2(c.wt[j], g[j], ma[j])));
+                    terms<ACT>(c, j, h, g);
+                    g[j] = fma2(c.a[j], g[j], fma2(h[j], mb[j], ma[j]));
                 }
                 *reinterpret_cast<Pack<T, VEC>*>(to) = pack<T, VEC>(g);
                 to += w.step;
@@ -1040,8 +1048,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
                 unpack<T, VEC>(slot[(2 * k + 1) * kGnThreads], g);
 #pragma unroll
                 for (int j = 0; j < P; j++) {
-                    h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
-                    g[j] = act_grad2<ACT>(g[j], fma2(h[j], c.wt[j], c.b[j]));
+                    terms<ACT>(c, j, h, g);
                     A[j] = add2(A[j], g[j]);
                     B[j] = fma2(g[j], h[j], B[j]);
                 }
@@ -1084,8 +1091,9 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
             float a1[2 * P], b1[2 * P];
             each_channel<VEC>(d, w, [&](int j, int, int g) {
                 const float2 m = stat[g - first];
-                a1[j] = -m.x;
-                b1[j] = -m.y;
+                const float r = rstd[n * d.G + g];
+                a1[j] = -m.x * r;
+                b1[j] = -m.y * r;
             });
             if (VEC == 1) a1[1] = b1[1] = 0.f;
 #pragma unroll
@@ -1121,10 +1129,8 @@ __global__ void __launch_bounds__(kGnThreads, kGnResidentGrad)
             if (k < w.steps) refill();
 #pragma unroll
             for (int j = 0; j < P; j++) {
-                h[j] = mul2(add2(h[j], c.mu[j]), c.r[j]);
-                g[j] = act_grad2<ACT>(g[j], fma2(h[j], c.wt[j], c.b[j]));
-                g[j] = mul2(c.r[j],
-                            fma2(h[j], mb[j], fma2(c.wt[j], g[j], ma[j])));
+                terms<ACT>(c, j, h, g);
+                g[j] = fma2(c.a[j], g[j], fma2(h[j], mb[j], ma[j]));
             }
             *reinterpret_cast<V*>(to) = pack<T, VEC>(g);
         }

@@ -239,3 +239,46 @@ def test_norm_and_step_refuse_a_trace(cuda):
         opt.step()
         n = optim.grad_norm([p.grad])
     assert int(opt.state[p]["step"]) == 1 and float(n) > 17.3
+
+
+# ---------------------------------------------------------------- relu's kink
+
+@pytest.mark.parametrize("rows", [23, 600])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_relu_gradient_where_its_output_is_not_zero(cuda, dtype, rows):
+    """The backward pass takes a value for positive exactly where the forward
+    pass did, to the last bit: biases put one value of each channel next to
+    zero. dbias is then a sum of powers of two, one for each positive value of
+    23 rows (the others have no gradient)."""
+    import torch
+
+    from opendressi_b200 import ops
+
+    dtype = getattr(torch, dtype)
+    c = 512
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.randn((1, rows, c), generator=g, device="cuda") + 2).to(dtype)
+    w = 1 + 0.3 * torch.randn(c, generator=g, device="cuda")
+    y, mean, rstd = ops.group_norm(x, 16, w, None, stats=True)
+    e = x[0].float() - mean.repeat_interleave(c // 16, 1)
+    z = e * (rstd.repeat_interleave(c // 16, 1) * w)
+    k = torch.arange(c, device="cuda") % 23
+    b = -z.gather(0, k[None]).reshape(-1).contiguous()
+    y, mean, rstd = ops.group_norm(x, 16, w, b, activation="none", stats=True)
+    small = (y[0].float().abs() < 1e-6).sum()
+    assert int(small) >= c // 4  # the biases reach the kink
+    dy = torch.zeros((1, rows, c), device="cuda")
+    dy[0, :23] = 2.0 ** (torch.arange(23, device="cuda") - 11)[:, None]
+    for want in ((True, True, True), (False, False, True)):
+        _, _, db = ops.group_norm_grad(dy.to(dtype), x, 16, w, b, mean, rstd,
+                                       activation="relu", want=want)
+        on = (db.double() * 2.0 ** 11).long()
+        relu = ops.group_norm(x, 16, w, b, activation="relu")[0, :23]
+        # a positive value may round to 0 in the output's type; f32 does not
+        bits = (y[0, :23].float() > 0) if dtype == torch.float32 else relu > 0
+        said = (on[None] >> torch.arange(23, device="cuda")[:, None]) & 1
+        if dtype == torch.float32:
+            assert torch.equal(said.bool(), bits)
+        else:
+            assert not (bits & ~said.bool()).any()
+            assert not ((y[0, :23].float() < 0) & said.bool()).any()
