@@ -2,6 +2,7 @@
 binding of its learning operators (_torch_binding.so) with g++.
 
     python -m opendressi_b200.build        # or opendressi_b200.build.build()
+    python -m opendressi_b200.build --library    # without the torch binding
 
 -fmad=false is required, not a tuning choice: the rasterizer's triangle-ID,
 coverage and distance outputs are bit-exact with the reference CPU code only
@@ -12,6 +13,8 @@ and denormals.
 
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import subprocess
 import sys
@@ -22,6 +25,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdressi_b200.so")
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 BINDING = os.path.join(HERE, "_torch_binding.so")
+OBJ_DIR = os.path.join(HERE, "_build")
+BINDING_STAMP = os.path.join(OBJ_DIR, "torch_binding.txt")
 SOURCES = ["capi.cu", "soft_raster.cu", "silhouette.cu", "hard_raster.cu",
            "fit.cu", "noalloc.cu",
            "antialias.cu", "texture.cu", "interp.cu", "regularize.cu",
@@ -80,56 +85,93 @@ def _stale() -> bool:
     return _older(LIB, [os.path.join(CSRC, f) for f in SOURCES + HEADERS])
 
 
-def _binding_command() -> list[str]:
-    """g++ for the torch binding: an extension module over torch's headers
-    and libdressi_b200.so (found beside it)."""
+def _torch_version() -> str | None:
+    """The installed torch's version; None where there is none."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    return importlib.metadata.version("torch")
+
+
+def _binding_commands() -> tuple[list[str], list[str]]:
+    """g++ to compile and to link the torch binding: an extension module over
+    torch's headers and libdressi_b200.so (found beside it)."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    lib = cpp_extension.library_paths()
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-            "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_torch_binding",
-            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
-            *[f"-isystem{p}" for p in cpp_extension.include_paths()],
-            f"-isystem{os.path.join(cuda, 'include')}",
-            f"-isystem{sysconfig.get_paths()['include']}", BINDING_SOURCE,
-            "-o", BINDING, *[f"-L{p}" for p in lib], f"-L{HERE}",
-            "-l:libdressi_b200.so", "-Wl,-rpath,$ORIGIN", "-lc10",
-            "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
-            "-ltorch_python"]
+    obj = os.path.join(OBJ_DIR, "torch_binding.o")
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+             "-DTORCH_EXTENSION_NAME=_torch_binding",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+             *[f"-isystem{p}" for p in cpp_extension.include_paths()],
+             f"-isystem{os.path.join(cuda, 'include')}",
+             f"-isystem{sysconfig.get_paths()['include']}", "-c",
+             BINDING_SOURCE, "-o", obj],
+            ["g++", "-shared", "-o", BINDING, obj,
+             *[f"-L{p}" for p in cpp_extension.library_paths()], f"-L{HERE}",
+             "-l:libdressi_b200.so", "-Wl,-rpath,$ORIGIN", "-lc10",
+             "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+             "-ltorch_python"])
 
 
-def _build_binding(force: bool, verbose: bool) -> None:
-    if not force and not _older(BINDING, [BINDING_SOURCE]):
-        return
-    cmd = _binding_command()
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    out = subprocess.run(cmd, capture_output=True, text=True)
-    if out.returncode != 0:
-        raise RuntimeError("g++ failed on torch_binding.cpp:\n" + out.stdout +
-                           out.stderr)
+def _binding_stamp() -> str:
+    """What a binding was built for: it loads into no other torch."""
+    return f"torch {_torch_version()}, {sys.implementation.cache_tag}\n"
 
 
-def build(force: bool = False, verbose: bool = False, jobs: int = 8) -> str:
-    """Compiles every translation unit, links the shared library and the
-    torch binding over it."""
-    _build_library(force, verbose, jobs)
-    _build_binding(force, verbose)
+def _binding_stale() -> bool:
+    try:
+        with open(BINDING_STAMP) as f:
+            if f.read() != _binding_stamp():
+                return True
+    except OSError:
+        return True
+    return _older(BINDING, [BINDING_SOURCE])
+
+
+def build(force: bool = False, verbose: bool = False, jobs: int = 8,
+          binding: bool = True) -> str:
+    """Compiles every translation unit and links the shared library and, where
+    torch is installed and `binding` is not False, the torch binding over it
+    (the library itself needs neither torch nor its headers)."""
+    link = compiled = None
+    if binding and _torch_version() is None:
+        print("torch is not installed: its binding of the learning operators "
+              "is left out", file=sys.stderr)
+    elif binding and (force or _binding_stale()):
+        compile_, link = _binding_commands()
+        os.makedirs(OBJ_DIR, exist_ok=True)
+        if verbose:
+            print(" ".join(compile_), file=sys.stderr)
+        compiled = subprocess.Popen(compile_, stdout=subprocess.PIPE,
+                                    stderr=subprocess.STDOUT)
+    try:
+        _build_library(force, verbose, jobs)
+    except BaseException:
+        if compiled:
+            compiled.kill()
+            compiled.communicate()
+        raise
+    if link:
+        _wait(("torch_binding.cpp", compiled))
+        out = subprocess.run(link, capture_output=True, text=True)
+        if out.returncode != 0:
+            raise RuntimeError("linking the torch binding failed:\n" +
+                               out.stdout + out.stderr)
+        with open(BINDING_STAMP, "w") as f:
+            f.write(_binding_stamp())
     return LIB
 
 
 def _build_library(force: bool, verbose: bool, jobs: int) -> None:
     if not force and not _stale():
         return
-    obj_dir = os.path.join(HERE, "_build")
-    os.makedirs(obj_dir, exist_ok=True)
+    os.makedirs(OBJ_DIR, exist_ok=True)
     objs, procs = [], []
     for src in SOURCES:
-        obj = os.path.join(obj_dir, os.path.splitext(src)[0] + ".o")
+        obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
         objs.append(obj)
         cmd = [nvcc(), *flags_for(src), "-c", os.path.join(CSRC, src), "-o",
                obj]
@@ -152,8 +194,9 @@ def _wait(item):
     src, p = item
     out, _ = p.communicate()
     if p.returncode != 0:
-        raise RuntimeError(f"nvcc failed on {src}:\n{out.decode()}")
+        raise RuntimeError(f"compiling {src} failed:\n{out.decode()}")
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose=True))
+    print(build(force="--force" in sys.argv, verbose=True,
+                binding="--library" not in sys.argv))
