@@ -1183,10 +1183,15 @@ struct GnPlan {
     int smem;        // bytes of a resident block
 };
 
-// A round of launches covers as many samples as stay in L2 between its two
-// passes (67 MB in one round take 45 us, in two 58, in four 90: a round's
-// launches cost 3 us, and what they do not read again is little).
-constexpr uint64_t kGnRoundBytes = 64ull << 20;
+// A round of launches covers as many samples as L2 (126 MB) about holds
+// between its two passes. 256x256x64 bf16, us: 9 views forward 64 with rounds
+// of 64 MiB at most and 49 with 128, 16 views 90 and 78, 8 views backward (two
+// images) 73 and 64. Over 34 shapes of 28 MiB to 2 GiB, forward and backward,
+// 128 MiB is never slower than 64 and takes up to 22% less. Above it no size
+// wins throughout: 192, 256, 512 MiB or no limit take up to 17% less again (9
+// views backward), 512 MiB also 29% more (300x64x64x128 bf16 backward, 430 us
+// against 333).
+constexpr uint64_t kGnRoundBytes = 128ull << 20;
 
 bool aligned(const void* p, size_t a) {
     return p == nullptr || reinterpret_cast<uintptr_t>(p) % a == 0;

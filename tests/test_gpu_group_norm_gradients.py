@@ -102,6 +102,27 @@ def test_more_samples_than_a_grid_counts(cuda):
                     check(t, ref, kind)
 
 
+def test_several_rounds_of_launches(cuda):
+    """Samples of 90 MB, more than one round takes together."""
+    import torch
+
+    from opendressi_b200 import torch_api as dr
+
+    x, dy, w, b = base.make(44, (3, 700, 801, 40), torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = dr.group_norm(x, 10, w, b, activation="silu")
+    grads = torch.autograd.grad(y, leaves, dy)
+    for k in range(3):  # sample by sample: the reference is large
+        xs = x.detach()[k:k + 1]
+        ref = reference(xs, w, b, 10, 1e-5, "silu", dy[k:k + 1])
+        check(y[k:k + 1], ref, "y")
+        check(grads[0][k:k + 1], ref, "dx")
+        sums = ref if k == 0 else {t: sums[t] + ref[t] for t in (
+            "dweight", "dbias", "dweight_err", "dbias_err")}
+    check(grads[1], sums, "dweight")
+    check(grads[2], sums, "dbias")
+
+
 @pytest.mark.parametrize("size", [1e-18, 1.0, 1e15])
 def test_no_eps(cuda, size):
     """With eps 0 the deviation alone scales: any size of values gives the
