@@ -38,7 +38,7 @@ namespace dressi {
 namespace {
 
 constexpr int kGnThreads = 256;
-constexpr int kGnSms = 148;
+constexpr int kGnSms = 148;  // of a B200; another number would cost time alone
 constexpr int kGnResident = 4;      // resident blocks an SM, forward
 constexpr int kGnResidentGrad = 2;  // backward
 
@@ -1308,9 +1308,11 @@ GnPlan make_plan(const GroupNormArgs& a, std::initializer_list<const void*> ps,
     };
     uint64_t chunks = chunks_of(grad ? 2 : 4);
     // Half as many blocks where a thread would take under 8 steps and then
-    // takes more: what a block does but once counts (forward, 3x127x193x96
-    // f16: 18.7 us with 6 steps, 16.7 with 12; 8x256x256x64 bf16: 45 us with
-    // 28, 53 with 56).
+    // takes more: what a block does but once counts. Of 180 f16 images (1, 3 or
+    // 8 samples of 16 to 384 channels, 2 to 48 MB) 36 meet this rule: 16 take 2
+    // to 19% less (1x110x111x384: 20.3 us and 16.5), 3 take 2 to 9% more
+    // (8x135x136x64: 20.7 and 22.5). With 8 steps or more, half the blocks take
+    // up to 18% more (3x128x128x384: 31.1 and 36.6).
     if (!grad && a.rows < lanes * 8 * chunks &&
         a.rows >= lanes * 8 * chunks_of(2))
         chunks = chunks_of(2);
