@@ -24,6 +24,11 @@ _BLOCK = 256  # values of 8-bit state that share a scale
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
+def _order(t) -> list:
+    """The strides of a tensor, where they count."""
+    return [s for s, n in zip(t.stride(), t.shape) if n != 1 and t.numel()]
+
+
 class _Pack:
     """The state of one parameter group: a flat tensor of each kind, every
     parameter at a multiple of 256 values of it."""
@@ -254,7 +259,8 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """Copies a state_dict() of an optimizer over like parameters into
         this one's own tensors (a learning rate that is a tensor here among
-        them, so that a captured step reads the loaded one)."""
+        them, so that a captured step reads the loaded one). 8-bit moments
+        need parameters in the same order of memory: their scales go by it."""
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
             if changed is not None:
@@ -277,6 +283,10 @@ class AdamW(torch.optim.Optimizer):
                             got[kind].dtype != t.dtype:
                         raise ValueError(f"the state's {kind} is not like "
                                          "this optimizer's")
+                    if t.dtype not in (torch.int32, torch.float32) and \
+                            _order(got[kind]) != _order(t):
+                        raise ValueError("the state's codes have scales of "
+                                         "another order of memory")
                     pairs.append((t, got[kind]))
         options = [self._loaded_options(g, old)
                    for g, old in zip(self.param_groups, groups)]

@@ -192,3 +192,47 @@ def test_a_host_learning_rate_is_checked_before_any_group_steps(cuda):
     with pytest.raises(ValueError):
         opt.step()
     assert torch.equal(p, before) and int(opt.state[p]["step"]) == 0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_loading_into_another_order_of_memory(cuda, bits):
+    """Codes go with the scale of 256 neighbours in memory: in another order
+    they would stand for other values. 32-bit moments go anywhere."""
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    t = torch.randn(64, 24, 3, 3, device="cuda")
+    t *= torch.logspace(-4, 0, 64, device="cuda")[:, None, None, None]
+    p = torch.nn.Parameter(t.clone())
+    q = torch.nn.Parameter(t.to(memory_format=torch.channels_last))
+    p.grad, q.grad = t.clone(), t.clone()
+    a, b = (optim.AdamW([x], state_bits=bits) for x in (p, q))
+    a.step()
+    if bits == 8:
+        with pytest.raises(ValueError, match="order"):
+            b.load_state_dict(a.state_dict())
+        assert not b.packed_state()["exp_avg"].float().any()
+        return
+    b.load_state_dict(a.state_dict())
+    q.data.copy_(p.data)
+    a.step()
+    b.step()
+    assert torch.equal(p, q)
+
+
+def test_loading_8_bit_state_of_odd_strides(cuda):
+    """Strides of extents of 1 do not count."""
+    torch = _torch()
+    from opendressi_b200 import optim
+
+    t = torch.randn(1, 5, 1, 700, device="cuda")
+    p = torch.nn.Parameter(t.clone())
+    q = torch.nn.Parameter(t.clone().as_strided(t.shape, (9, 700, 1, 1)))
+    p.grad, q.grad = t.clone(), t.clone()
+    a, b = (optim.AdamW([x], state_bits=8, seed=5) for x in (p, q))
+    a.step()
+    b.load_state_dict(a.state_dict())
+    q.data.copy_(p.data)
+    a.step()
+    b.step()
+    assert torch.equal(p, q)
