@@ -362,7 +362,8 @@ int dressi_group_norm(const dressi_group_norm_desc* d, const void* x,
                       size_t workspace_bytes, void* stream);
 
 /* The gradients for dy, from x and the statistics of the forward call. dx,
- * dweight and dbias are overwritten; each may be NULL. Repeats bit for bit. */
+ * dweight and dbias are overwritten, must not overlap an input, and may each be
+ * NULL. Repeats bit for bit. */
 int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
                            const void* x, const float* weight,
                            const float* bias, const float* mean,
@@ -374,7 +375,8 @@ int dressi_group_norm_grad(const dressi_group_norm_desc* d, const void* dy,
 int dressi_grad_norm_workspace(size_t* bytes);
 
 /* out[0] = sqrt(sum of squares over n_tensors tensors), summed in 64 bits in
- * an order that the sizes alone give. tensors, numel and dtypes are host
+ * an order that the sizes, the tensors' alignments and the device's number of
+ * SMs give. tensors, numel and dtypes are host
  * arrays (read before the call returns) of device addresses, lengths and
  * element types. The workspace is aligned to 8 bytes. */
 int dressi_grad_norm(uint32_t n_tensors, const void* const* tensors,

@@ -741,7 +741,8 @@ def group_norm_grad(dy, x, num_groups: int, weight, bias, mean, rstd,
 def grad_norm(tensors, out=None) -> torch.Tensor:
     """sqrt of the sum of squares over all tensors (float32, float16 or
     bfloat16, of any shapes, on one device) as a 0-dim float32 CUDA tensor;
-    summed in 64 bits in an order that the sizes alone give."""
+    summed in 64 bits, in an order that the sizes, the alignments and the
+    device give. `out`, if given, holds one float32 and needs no gradient."""
     if isinstance(tensors, torch.Tensor):
         tensors = [tensors]
     return binding().grad_norm(list(tensors), out)

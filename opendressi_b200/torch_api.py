@@ -720,7 +720,8 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5,
     ("none", "relu" or "silu"). x is float32, float16 or bfloat16 and so is
     the result; statistics are taken in 32 bits and more. A channels-last
     tensor of shape [N, C, H, W] is given as x.permute(0, 2, 3, 1), which
-    copies nothing. Differentiable once, w.r.t. x, weight and bias, in reverse
+    copies nothing. Made for samples of some KB and more: a table of very many
+    tiny ones is slow. Differentiable once, w.r.t. x, weight and bias, in reverse
     mode (an input with a forward-mode tangent is refused)."""
     if not torch.compiler.is_compiling():
         # the operator below with its autograd in C++, unless a trace or a
