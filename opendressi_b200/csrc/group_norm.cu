@@ -13,8 +13,9 @@
 // wants it (8x256x256x64 bf16 forward: 45 us, against 20.5 for its bytes at the
 // copy rate; 2x1024x1024x64 bf16 with its gradient: 414 us, a sample being
 // larger than L2). Samples of a few values are not what it is made for: a block
-// takes them one by one (10^6 x 32 f32: 6.6 ms, 21 ms backward). Statistics are 32-bit per thread about the thread's own
-// first value (no cancellation where |mean| >> deviation), merged in 32 bits
+// takes them one by one (10^6 x 32 f32: 6.6 ms, 21 ms backward). Statistics are
+// 32-bit per thread about the mean of the thread's values so far (no
+// cancellation where |mean| >> deviation), merged in 32 bits
 // within a block as distances from a common value and in 64 bits between
 // blocks; sums are taken in a fixed order, so reruns give the same bits.
 //
@@ -401,19 +402,48 @@ __device__ __forceinline__ Two act_grad2(Two dy, Two z) {
 // (the pairwise update of Chan, Golub and LeVeque, all at once). Means enter
 // as distances from one of them: the square of a mean of many deviations would
 // leave no digits of the variance in 32 bits.
+//
+// Where the first value is far from the others (a bright corner), a sum of
+// squares about it is N times the variance's: so the sums are moved to the mean
+// so far after 4, 16, 64, ... values. Squares are then at most 4 times what they
+// are about the mean of all: of 4 n values, with d from the first n's mean to
+// the others', they sum up to m about their own mean, 3/4 n d^2 or more, and to
+// m + 9/4 n d^2 about the first n's.
 template <int VEC>
 struct ThreadMoments {
     static constexpr int P = kPairs<VEC>;
-    Two k[P], s1[P], s2[P];
+    Two k[P], s1[P], s2[P];  // -centre, sums of distances from it and squares
+    uint32_t left;           // values until the next move
+    float count;             // values that there are then
 
+    // At the first value, which counts as met or comes again.
     template <typename T>
-    __device__ __forceinline__ void begin(const Pack<T, VEC>& first) {
+    __device__ __forceinline__ void begin(const Pack<T, VEC>& first,
+                                          bool met) {
         unpack<T, VEC>(first, k);
 #pragma unroll
         for (int j = 0; j < P; j++) {
             k[j] = mul2(k[j], two(-1.f));
             s1[j] = s2[j] = two(0.f);
         }
+        left = met ? 3 : 4;
+        count = 4.f;
+    }
+    // The sums about c + d from those about c, d the values' mean distance.
+    __device__ __forceinline__ void move() {
+        const float inv = -1.f / count;
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            const Two old = k[j];
+            k[j] = fma2(s1[j], two(inv), old);
+            const Two d = fma2(k[j], two(-1.f), old);  // as it was rounded
+            const Two nd = mul2(d, two(-count));
+            s2[j] = fma2(mul2(d, two(-1.f)),
+                         add2(s1[j], add2(s1[j], nd)), s2[j]);
+            s1[j] = add2(s1[j], nd);
+        }
+        left = 3 * uint32_t(count);
+        count *= 4.f;
     }
     template <typename T>
     __device__ __forceinline__ void add(const Pack<T, VEC>& v) {
@@ -425,6 +455,7 @@ struct ThreadMoments {
             s1[j] = add2(s1[j], e[j]);
             s2[j] = fma2(e[j], e[j], s2[j]);
         }
+        if (--left == 0) move();
     }
     // (mean, sum of squares) of each run of channels to sm.
     __device__ __forceinline__ void put(uint32_t steps, int run, float2* sm) {
@@ -539,7 +570,7 @@ __global__ void __launch_bounds__(kGnThreads)
         const T* own = x + n * d.rows * d.C + w.base;
         walk_over<T, VEC, 1>(
                 own, static_cast<const T*>(nullptr), w.step, w.steps, ring,
-                [&] { m.begin(load_pack<T, VEC>(own)); },
+                [&] { m.begin(load_pack<T, VEC>(own), false); },
                 [&](const Pack<T, VEC>& v, const Pack<T, VEC>&) { m.add(v); });
     }
     // the ring is free once every thread has left it
@@ -713,7 +744,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnResident)
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (w.steps > 0) {
             ThreadMoments<VEC> m;
-            m.begin(*slot);
+            m.begin(*slot, true);
             for (uint32_t k = 1; k < w.steps; k++) m.add(slot[k * kGnThreads]);
             m.put(w.steps, d.run, sm);
         }

@@ -123,6 +123,42 @@ def test_several_rounds_of_launches(cuda):
     check(grads[2], sums, "dbias")
 
 
+@pytest.mark.parametrize("far", [1e2, 1e4, 1e6])
+@pytest.mark.parametrize("shape,groups,steps", [
+    ((1, 64, 64, 32), 8, 4), ((3, 40, 40, 16), 4, 13),
+    ((8, 256, 256, 64), 16, 56), ((1, 2048, 2048, 32), 8, 222),
+    ((2, 1201, 1013, 3), 1, 139)])
+def test_values_far_from_the_others(cuda, shape, groups, steps, far):
+    """A bright corner, the first row, the last row: what a thread meets first
+    must not cancel its sums. A sum of squares about a centre is at most 4
+    times what it is about the mean; its `steps` roundings of 2^-24 (of either
+    sign) add up to sqrt(steps) of them, the rest is the 64 of `base`, which
+    cover 32."""
+    import torch
+
+    from opendressi_b200 import ops
+
+    tol = base.K * base.U * max(1.0, math.sqrt(steps / 32.0))
+    for where in ((0, 0), (0,), (-1,), (0, slice(None, None, 7))):
+        g = torch.Generator(device="cuda").manual_seed(9)
+        x = torch.randn(shape, generator=g, device="cuda")
+        x[(slice(None), *where)] += far
+        y, mean, rstd = ops.group_norm(x, groups, stats=True)
+        n, c = shape[0], shape[-1] // groups
+        for k in range(groups):
+            d = x[..., k * c:(k + 1) * c].reshape(n, -1).double()
+            mu = d.mean(1, keepdim=True)
+            dev = (((d - mu) ** 2).mean(1) + 1e-5).sqrt()
+            assert ((rstd[:, k].double() * dev - 1).abs() <= tol).all()
+            # 8 roundings of the largest distance from it (the proof stands in
+            # test_gpu_group_norm.py: a thread's mean is its centre and a mean
+            # of distances from there, 3 roundings of at most twice that, and
+            # those of the sum) and the mean's own
+            reach = (d - mu).abs().amax(1)
+            assert ((mean[:, k].double() - mu[:, 0]).abs() <=
+                    base.U * (8 * reach + mu[:, 0].abs())).all()
+
+
 @pytest.mark.parametrize("size", [1e-18, 1.0, 1e15])
 def test_no_eps(cuda, size):
     """With eps 0 the deviation alone scales: any size of values gives the
