@@ -66,6 +66,9 @@ void on_cuda(const Tensor& t, const char* name) {
         refuse(std::string(name) + " must be a dense CUDA tensor");
 }
 
+// t's values packed in memory, a lazy negation (of an imaginary part) done.
+Tensor packed(const Tensor& t) { return t.contiguous().resolve_neg(); }
+
 void* stream_of(const Tensor& t) {
     return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
@@ -96,7 +99,7 @@ Tensor table(const Tensor& t, const char* name, const Tensor& x) {
         refuse(std::string(name) + " must be [" + std::to_string(x.size(-1)) +
                "] on " + x.device().str() + ", got " + shape_of(t) + " on " +
                t.device().str());
-    return t.contiguous();
+    return packed(t);
 }
 
 int activation_of(const std::string& name) {
@@ -135,7 +138,7 @@ std::vector<Tensor> norm_forward(const Tensor& x_, int64_t groups,
                                  const Tensor& weight_, const Tensor& bias_,
                                  double eps, int activation, bool stats) {
     const dressi_group_norm_desc d = norm_desc(x_, groups, eps, activation);
-    const Tensor x = x_.contiguous();
+    const Tensor x = packed(x_);
     const Tensor weight = table(weight_, "weight", x);
     const Tensor bias = table(bias_, "bias", x);
     Tensor y = at::empty_like(x), mean, rstd;
@@ -171,7 +174,7 @@ std::vector<Tensor> norm_backward(const Tensor& dy_, const Tensor& x_,
     if (dy_.sizes() != x_.sizes() || dy_.scalar_type() != x_.scalar_type() ||
         dy_.device() != x_.device())
         refuse("dy must be like x");
-    const Tensor x = x_.contiguous(), dy = dy_.contiguous();
+    const Tensor x = packed(x_), dy = packed(dy_);
     const Tensor weight = table(weight_, "weight", x);
     const Tensor bias = table(bias_, "bias", x);
     for (const Tensor* t : {&mean_, &rstd_}) {
@@ -182,7 +185,7 @@ std::vector<Tensor> norm_backward(const Tensor& dy_, const Tensor& x_,
             refuse("mean and rstd must be float32 [N, groups] on " +
                    x.device().str() + ", got " + shape_of(*t));
     }
-    const Tensor mean = mean_.contiguous(), rstd = rstd_.contiguous();
+    const Tensor mean = packed(mean_), rstd = packed(rstd_);
     const auto opt = x.options().dtype(at::kFloat);
     Tensor dx, dw, db;
     if (want_x) dx = at::empty_like(x);
@@ -374,7 +377,7 @@ Tensor grad_norm(const std::vector<Tensor>& tensors,
         out = *out_;
         on_cuda(out, "out");
         if (out.scalar_type() != at::kFloat || out.numel() != 1 ||
-            out.device() != dev)
+            out.device() != dev || out.is_neg())
             refuse("out must hold one float32 on " + dev.str());
         if (out.requires_grad()) refuse("out requires a gradient");
     } else {
@@ -438,7 +441,7 @@ struct Pack {
             // as many values and the same strides could still be a view that
             // is not dense: the kernel writes numel values in a row
             if (dtype_of(r.p, "parameter") != r.dtype ||
-                r.p.device() != dev ||
+                r.p.device() != dev || r.p.is_neg() ||
                 r.p.sizes() != at::IntArrayRef(r.sizes) ||
                 r.p.strides() != at::IntArrayRef(r.strides)) {
                 refuse("a parameter changed its type, shape or device; make a "
@@ -451,8 +454,9 @@ struct Pack {
                 r.g.sizes() != r.p.sizes() || r.g.device() != dev) {
                 refuse("a gradient must be dense and like its parameter");
             }
-            if (r.g.strides() != r.p.strides() &&
-                !(r.g.is_contiguous() && r.p.is_contiguous())) {
+            if (r.g.is_neg() ||
+                (r.g.strides() != r.p.strides() &&
+                 !(r.g.is_contiguous() && r.p.is_contiguous()))) {
                 r.g = at::empty_strided(r.p.sizes(), r.p.strides(),
                                         r.p.options())
                               .copy_(r.g);
@@ -554,7 +558,9 @@ void adamw_step(const std::vector<Pack*>& packs,
 }
 
 // Whether the values of t fill its extent in memory once, in some order.
-bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
+bool dense(const Tensor& t) {
+    return t.is_non_overlapping_and_dense() && !t.is_neg();
+}
 
 }  // namespace
 

@@ -282,3 +282,50 @@ def test_relu_gradient_where_its_output_is_not_zero(cuda, dtype, rows):
         else:
             assert not (bits & ~said.bool()).any()
             assert not ((y[0, :23].float() < 0) & said.bool()).any()
+
+
+def test_lazily_negated_tensors(cuda):
+    """Tensors whose sign is a bit of theirs (the imaginary part of a lazily
+    conjugated tensor): their values count, not what memory holds."""
+    import torch
+
+    from opendressi_b200 import ops, optim, torch_api as dr
+
+    x, w, b = inputs(7)
+    dy = torch.randn_like(x)
+    nx, nw, nb, ndy = (torch._neg_view(-t) for t in (x, w, b, dy))
+    assert nx.is_neg() and nx.is_contiguous() and torch.equal(nx, x)
+    y, mean, rstd = ops.group_norm(x, 3, w, b, activation="silu", stats=True)
+    for got in (ops.group_norm(nx, 3, nw, nb, activation="silu"),
+                dr.group_norm(nx, 3, w, b, activation="silu"),
+                dr.group_norm(x, 3, nw, nb, activation="silu")):
+        assert torch.equal(got, y)
+    want = ops.group_norm_grad(dy, x, 3, w, b, mean, rstd, activation="silu")
+    for got in (ops.group_norm_grad(ndy, nx, 3, nw, nb, torch._neg_view(-mean),
+                                    torch._neg_view(-rstd),
+                                    activation="silu"),):
+        for a, e in zip(got, want):
+            assert torch.equal(a, e)
+    leaf = x.clone().requires_grad_(True)
+    (gx,) = torch.autograd.grad(dr.group_norm(leaf, 3, w, b,
+                                              activation="silu"), leaf, ndy)
+    assert torch.equal(gx, want[0])
+
+    p, q = leaves((300,), (300,))
+    with torch.no_grad():
+        q.copy_(p)
+    p.grad = torch.randn_like(p)
+    q.grad = torch._neg_view(-p.grad)
+    for t in (p, q):
+        optim.AdamW([t], max_norm=1.0).step()
+    assert torch.equal(p, q)
+    from opendressi_b200 import DressiError
+
+    with pytest.raises(DressiError):
+        optim.AdamW([torch.nn.Parameter(torch._neg_view(x))])
+    opt = optim.AdamW([p])
+    p.data = torch._neg_view(p.detach())
+    for call in (opt.step, lambda: optim.grad_norm(
+            [x], out=torch._neg_view(torch.ones((), device="cuda")))):
+        with pytest.raises(DressiError):
+            call()
